@@ -1,0 +1,419 @@
+// Paged attention of single next tokens whose requests share a prefix (a system prompt, the beams of one search).
+//
+// Rows (one token each) come in groups: the rows group_start[g] .. group_start[g + 1] - 1 share the positions
+// [0, prefix_len[g]), which lie in the pages of block-table row prefix_slot[g].  A position behind them lies in the
+// pages of the row's own request, or, with a history, in those of the member of the group that wrote it: the beams of a search
+// keep their keys where they were written, and what a beam inherits is a list of writers (history[slot][n] is the
+// member that wrote position prefix_len + n; the row's own position is always its own).  A row at position pos sees
+// [max(0, pos - window + 1), pos].
+//
+// The query heads of all members over one key/value head are the rows of one matrix product over the shared keys, so
+// these are read once for the group instead of once for every member: out = sum_j softmax(s)_j v_j is taken apart into the
+// part over the shared positions and the part over the others, each with its maximum m, its sum l of 2^(s - m) and its
+// unnormalised output o, all in float32, and the parts are added up as sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
+//
+// This file: the general kernel (float32 or bfloat16, any head size up to 256) for both parts, and the one that adds
+// parts up.
+#include "mma_utils.cuh"
+
+namespace tk {
+
+struct SharedParams {
+  const void* q;                // [rows, n_q_heads, d]
+  void* out;                    // [rows, n_q_heads, dv]
+  const void* k_cache;          // [num_pages, n_kv_heads, page_size, d]
+  const void* v_cache;          // [num_pages, n_kv_heads, page_size, dv]
+  const int* group_start;       // [n_groups + 1]
+  const int* prefix_slot;       // [n_groups]
+  const int* prefix_len;        // [n_groups]
+  const int* positions;         // [rows]
+  const int* req_slot;          // [rows]
+  const int* block_table;       // [max_slots, max_pages]
+  const unsigned char* history; // [max_slots, history_ld] or null
+  const float* sinks;           // [n_q_heads] or null
+  float* part_o;                // [rows, n_q_heads, n_parts, dv]
+  float* part_ml;               // [rows, n_q_heads, n_parts, 2]
+  int* err;
+  int n_rows, n_groups, max_members, n_q_heads, n_kv_heads, d, dv, page_size, max_pages, num_pages, max_slots, history_ld, window;
+  int n_shared, n_own, n_parts; // parts of the shared and of the other positions; n_parts = n_shared + n_own
+  int wide_k, wide_v;           // rows of queries and keys, of values, can be read four elements at a time
+  float scale_log2, cap_log2, inv_cap;
+};
+
+// The group that holds a row: the last one that starts at or before it.
+__device__ __forceinline__ int group_of_row(const SharedParams& p, int row) {
+  int lo = 0, hi = p.n_groups - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.group_start[mid] <= row) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Rows of group g, cut to what exists.
+__device__ __forceinline__ int2 group_rows(const SharedParams& p, int g) {
+  const int a = max(0, min(p.n_rows, p.group_start[g]));
+  const int b = max(a, min(p.n_rows, p.group_start[g + 1]));
+  return make_int2(a, min(b, a + p.max_members));
+}
+
+__device__ __forceinline__ int checked_slot(const SharedParams& p, int slot, int row) {
+  if (slot >= 0 && slot < p.max_slots) return slot;
+  set_error(p.err, kErrRequest, row, slot, p.max_slots);
+  return -1;
+}
+
+// Place of a position in the pools: (page * n_kv_heads + head) * page_size + offset, -1 for one that has no page.
+__device__ __forceinline__ long long pool_row(const SharedParams& p, int slot, int pos, int hkv, int row) {
+  const int pidx = pos / p.page_size;
+  const int page = (slot >= 0 && pidx < p.max_pages) ? p.block_table[(size_t)slot * p.max_pages + pidx] : -1;
+  if (page < 0 || page >= p.num_pages) {
+    if (slot >= 0) set_error(p.err, kErrPage, row, pidx, page);
+    return -1;
+  }
+  return ((long long)page * p.n_kv_heads + hkv) * p.page_size + pos % p.page_size;
+}
+
+// The slot that holds position `pos` (behind the shared ones) of row `row`.
+__device__ __forceinline__ int writer_slot(const SharedParams& p, int row, int slot, int pos, int own_pos, int prefix, int2 rows) {
+  if (p.history == nullptr || pos == own_pos || slot < 0) return slot;
+  const int n = pos - prefix;
+  if (n >= p.history_ld) { set_error(p.err, kErrPosition, row, pos, p.history_ld); return -1; }
+  const int member = p.history[(size_t)slot * p.history_ld + n];
+  if (member >= rows.y - rows.x) { set_error(p.err, kErrRequest, row, member, rows.y - rows.x); return -1; }
+  return checked_slot(p, p.req_slot[rows.x + member], row);
+}
+
+// Whether the row belongs to a group as it should; where not, its shared parts are marked as empty here (head >= 0: for that
+// head), since no block of the shared positions does it, and an error is set.
+__device__ __forceinline__ bool row_has_group(const SharedParams& p, int row, int2 rows, int prefix, int head) {
+  if (row >= rows.x && row < rows.y && (p.n_shared > 0 || prefix == 0)) return true;
+  set_error(p.err, kErrRequest, row, p.max_members, prefix);
+  if (head >= 0) {
+    float* ml = p.part_ml + 2 * ((size_t)row * p.n_q_heads + head) * p.n_parts;
+    for (int i = 0; i < p.n_shared; ++i) { ml[2 * i] = -INFINITY; ml[2 * i + 1] = 0.0f; }
+  }
+  return false;
+}
+
+// What a row sees: [lo, pos]; bad positions see nothing.
+struct RowSpan { int pos, lo; };
+__device__ __forceinline__ RowSpan row_span(const SharedParams& p, int row) {
+  const int pos = p.positions[row];
+  if (pos < 0) { set_error(p.err, kErrPosition, row, pos, 0); return {-1, 0}; }
+  return {pos, first_visible(pos, p.window, 0)};
+}
+
+// ---- general kernel -----------------------------------------------------------------------------------------------
+//
+// A block takes up to 32 (row, query head) pairs over one key/value head and a range of keys: of the shared positions, where
+// the pairs are those of a tile of the group's members, or of one row's others.  Tiles of 32 keys go through shared memory as
+// float32; warp w holds four pairs: a lane computes the four scores of its key, then owns four (or eight) columns of the output.
+constexpr int kShRows = 32;
+constexpr int kShKeys = 32;
+constexpr int kShThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ void load_row(float* dst, const T* src, int n, bool wide, int lane0, int lanes) {
+  if (wide) {
+    for (int c = lane0; c < n / 4; c += lanes) {
+      float4 f;
+      if constexpr (sizeof(T) == 4) {
+        f = *reinterpret_cast<const float4*>(src + 4 * c);
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(src + 4 * c);
+        const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&u.x), b = *reinterpret_cast<const __nv_bfloat162*>(&u.y);
+        f = make_float4(__bfloat162float(a.x), __bfloat162float(a.y), __bfloat162float(b.x), __bfloat162float(b.y));
+      }
+      *reinterpret_cast<float4*>(dst + 4 * c) = f;
+    }
+  } else {
+    for (int c = lane0; c < n; c += lanes) dst[c] = to_f32<T>(src[c]);
+  }
+}
+
+template <typename T, int kChunks>       // kChunks: 128-column chunks of a value row
+__global__ void __launch_bounds__(kShThreads) shared_parts_kernel(SharedParams p, int row_tiles, int n_shared_blocks) {
+  pdl_trigger();
+  extern __shared__ __align__(16) float s_mem[];
+  __shared__ long long s_row[kShKeys];
+  __shared__ int s_pos[kShRows], s_lo[kShRows], s_tok[kShRows], s_head[kShRows];
+  __shared__ float s_p[kShRows / 4][kShKeys][4];
+  const int dp = (p.d + 3) / 4 * 4, dvp = (p.dv + 3) / 4 * 4;
+  const int ldk = dp + 4;
+  float* s_q = s_mem;                          // [kShRows][dp]
+  float* s_k = s_q + kShRows * dp;             // [kShKeys][ldk]
+  float* s_v = s_k + kShKeys * ldk;            // [kShKeys][dvp]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = p.n_q_heads / p.n_kv_heads;
+  pdl_wait();
+
+  // ---- what this block does ------------------------------------------------------------------------------------
+  const bool shared = (int)blockIdx.x < n_shared_blocks;
+  int b = shared ? (int)blockIdx.x : (int)blockIdx.x - n_shared_blocks;
+  const int splits = shared ? p.n_shared : p.n_own;
+  const int split = b % splits; b /= splits;
+  const int hkv = b % p.n_kv_heads; b /= p.n_kv_heads;
+  const int tile = b % row_tiles; b /= row_tiles;
+  int g, first_pair, n_pairs, prefix, slot = -1, own_row = -1;
+  int2 rows;
+  if (shared) {
+    g = b;
+    rows = group_rows(p, g);
+    first_pair = tile * kShRows;
+    n_pairs = min(kShRows, (rows.y - rows.x) * per - first_pair);
+    prefix = max(0, p.prefix_len[g]);
+    slot = prefix > 0 && n_pairs > 0 ? checked_slot(p, p.prefix_slot[g], rows.x) : -1;
+  } else {
+    own_row = b;
+    g = group_of_row(p, own_row);
+    rows = group_rows(p, g);
+    first_pair = tile * kShRows;
+    n_pairs = min(kShRows, per - first_pair);
+    prefix = max(0, p.prefix_len[g]);
+    slot = checked_slot(p, p.req_slot[own_row], own_row);
+  }
+  if (n_pairs <= 0) return;
+  if (!shared && !row_has_group(p, own_row, rows, prefix, split == 0 && tid < n_pairs ? hkv * per + first_pair + tid : -1)) slot = -1;
+  if (tid < kShRows) {
+    const int pair = first_pair + tid;
+    const int row = shared ? rows.x + pair / per : own_row;
+    s_tok[tid] = row;
+    s_head[tid] = hkv * per + pair % per;
+    RowSpan sp = {-1, 0};
+    if (tid < n_pairs) sp = row_span(p, row);
+    s_pos[tid] = sp.pos;
+    s_lo[tid] = sp.lo;
+  }
+  __syncthreads();
+  int lo = 0x7fffffff, hi = -1;                // keys that any of the pairs sees
+  for (int i = 0; i < n_pairs; ++i) {
+    if (s_pos[i] >= 0) { lo = min(lo, s_lo[i]); hi = max(hi, s_pos[i]); }
+  }
+  if (shared) hi = min(hi, prefix - 1); else lo = max(lo, prefix);
+  if (slot < 0) hi = -1;
+  const int n_keys = hi >= lo ? hi - lo + 1 : 0;
+  const int n_tiles = (n_keys + kShKeys - 1) / kShKeys;
+  const int per_split = (n_tiles + splits - 1) / splits;
+  const int t0 = split * per_split, t1 = min(n_tiles, t0 + per_split);
+
+  const bool wide_k = p.wide_k, wide_v = p.wide_v;
+  if (t0 < t1) {
+    for (int i = warp; i < n_pairs; i += kShThreads / 32) {
+      load_row<T>(s_q + i * dp, (const T*)p.q + ((size_t)s_tok[i] * p.n_q_heads + s_head[i]) * p.d, p.d, wide_k, lane, 32);
+      for (int c = p.d + lane; c < dp; c += 32) s_q[i * dp + c] = 0.0f;
+    }
+  }
+  float m[4], l[4], acc[4][4 * kChunks];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    m[r] = -INFINITY; l[r] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4 * kChunks; ++c) acc[r][c] = 0.0f;
+  }
+  const bool active = 4 * warp < n_pairs;
+  for (int t = t0; t < t1; ++t) {
+    const int key0 = lo + t * kShKeys;
+    __syncthreads();                           // the tile before is done with
+    if (tid < kShKeys) {
+      const int key = key0 + tid;
+      long long at = -1;
+      if (key <= hi) {
+        const int from = shared ? slot : writer_slot(p, own_row, slot, key, s_pos[0], prefix, rows);
+        at = pool_row(p, from, key, hkv, s_tok[0]);
+      }
+      s_row[tid] = at;
+    }
+    __syncthreads();
+    for (int i = warp; i < kShKeys; i += kShThreads / 32) {
+      const long long at = s_row[i];
+      if (at >= 0) {
+        load_row<T>(s_k + i * ldk, (const T*)p.k_cache + at * p.d, p.d, wide_k, lane, 32);
+        load_row<T>(s_v + i * dvp, (const T*)p.v_cache + at * p.dv, p.dv, wide_v, lane, 32);
+        for (int c = p.d + lane; c < dp; c += 32) s_k[i * ldk + c] = 0.0f;
+      } else {
+        // a key that is not there: nothing that lies in its place may reach the result
+        for (int c = lane; c < dp; c += 32) s_k[i * ldk + c] = 0.0f;
+        for (int c = lane; c < dvp; c += 32) s_v[i * dvp + c] = 0.0f;
+      }
+    }
+    __syncthreads();
+    if (active) {
+      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const float* kr = s_k + lane * ldk;
+      const float* qr = s_q + 4 * warp * dp;
+      for (int c = 0; c < dp; c += 4) {
+        const float4 kv = *reinterpret_cast<const float4*>(kr + c);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float4 qv = *reinterpret_cast<const float4*>(qr + r * dp + c);
+          s[r] = fmaf(qv.x, kv.x, s[r]); s[r] = fmaf(qv.y, kv.y, s[r]);
+          s[r] = fmaf(qv.z, kv.z, s[r]); s[r] = fmaf(qv.w, kv.w, s[r]);
+        }
+      }
+      const int key = key0 + lane;
+      float4 prob;
+      float* pr = &prob.x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 4 * warp + r;
+        const bool seen = i < n_pairs && s_row[lane] >= 0 && key <= s_pos[i] && key >= s_lo[i];
+        const float x = seen ? capped_score_log2(s[r], p.scale_log2, p.cap_log2, p.inv_cap) : -INFINITY;
+        const float m_new = fmaxf(m[r], warp_max(x));
+        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+        const float corr = exp2f(m[r] - m_use);
+        m[r] = m_new;
+        pr[r] = exp2f(x - m_use);
+        l[r] = l[r] * corr + warp_sum(pr[r]);
+#pragma unroll
+        for (int c = 0; c < 4 * kChunks; ++c) acc[r][c] *= corr;
+      }
+      *reinterpret_cast<float4*>(&s_p[warp][lane][0]) = prob;
+      __syncwarp();
+#pragma unroll
+      for (int ch = 0; ch < kChunks; ++ch) {
+        const int col = ch * 128 + lane * 4;
+        if (col < dvp) {
+          for (int j = 0; j < kShKeys; ++j) {
+            const float4 w = *reinterpret_cast<const float4*>(&s_p[warp][j][0]);
+            const float4 vv = *reinterpret_cast<const float4*>(s_v + j * dvp + col);
+            const float wr[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              acc[r][4 * ch] = fmaf(wr[r], vv.x, acc[r][4 * ch]);
+              acc[r][4 * ch + 1] = fmaf(wr[r], vv.y, acc[r][4 * ch + 1]);
+              acc[r][4 * ch + 2] = fmaf(wr[r], vv.z, acc[r][4 * ch + 2]);
+              acc[r][4 * ch + 3] = fmaf(wr[r], vv.w, acc[r][4 * ch + 3]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
+  if (!active) return;
+  const int part = shared ? split : p.n_shared + split;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = 4 * warp + r;
+    if (i >= n_pairs) break;
+    const size_t at = ((size_t)s_tok[i] * p.n_q_heads + s_head[i]) * p.n_parts + part;
+    if (lane == 0) { p.part_ml[2 * at] = m[r]; p.part_ml[2 * at + 1] = l[r]; }
+    if (l[r] > 0.0f) {                         // a part without keys has no output that anybody reads
+#pragma unroll
+      for (int ch = 0; ch < kChunks; ++ch) {
+        const int col = ch * 128 + lane * 4;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (col + c < p.dv) p.part_o[at * p.dv + col + c] = acc[r][4 * ch + c];
+        }
+      }
+    }
+  }
+}
+
+// ---- parts added up -------------------------------------------------------------------------------------------------
+// A warp per (row, query head); a row that sees nothing is zero.
+constexpr int kMergeWarps = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(kMergeWarps * 32) shared_merge_kernel(SharedParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long pair = (long long)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+  if (pair >= (long long)p.n_rows * p.n_q_heads) return;
+  const int head = (int)(pair % p.n_q_heads);
+  const float* ml = p.part_ml + 2 * pair * p.n_parts;
+  float m_all = -INFINITY;
+  for (int i = lane; i < p.n_parts; i += 32) m_all = fmaxf(m_all, __ldcg(ml + 2 * i));
+  m_all = warp_max(m_all);
+  float l_all = 0.0f;
+  for (int i = lane; i < p.n_parts; i += 32) {
+    const float l = __ldcg(ml + 2 * i + 1);
+    if (l > 0.0f) l_all += l * exp2f(__ldcg(ml + 2 * i) - m_all);
+  }
+  l_all = warp_sum(l_all);
+  const float inv = l_all > 0.0f ? 1.0f / (l_all + sink_term_log2(p.sinks, head, m_all)) : 0.0f;
+  T* out = (T*)p.out + pair * p.dv;
+  const float* o = p.part_o + (size_t)pair * p.n_parts * p.dv;
+  for (int c0 = 0; c0 < p.dv; c0 += 32) {
+    const int c = c0 + lane;
+    float acc = 0.0f;
+    for (int i = 0; i < p.n_parts; ++i) {
+      const float l = __ldcg(ml + 2 * i + 1);
+      if (l > 0.0f && c < p.dv) acc += __ldcg(o + (size_t)i * p.dv + c) * exp2f(__ldcg(ml + 2 * i) - m_all);
+    }
+    if (c < p.dv) out[c] = from_f32<T>(acc * inv);
+  }
+}
+
+template <typename T>
+static int launch_general(const SharedParams& p, cudaStream_t stream) {
+  const int per = p.n_q_heads / p.n_kv_heads;
+  const int dp = (p.d + 3) / 4 * 4, dvp = (p.dv + 3) / 4 * 4;
+  const size_t smem = sizeof(float) * ((size_t)kShRows * dp + (size_t)kShKeys * (dp + 4) + (size_t)kShKeys * dvp);
+  const int shared_tiles = (p.max_members * per + kShRows - 1) / kShRows, own_tiles = (per + kShRows - 1) / kShRows;
+  const long long n_shared = (long long)p.n_groups * shared_tiles * p.n_kv_heads * p.n_shared;
+  const long long n_own = (long long)p.n_rows * own_tiles * p.n_kv_heads * p.n_own;
+  if (n_shared > 0x7fffffffLL || n_own > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  auto run = [&](auto kernel) -> int {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    if (n_shared > 0) {
+      e = launch(kernel, dim3((unsigned)n_shared), dim3(kShThreads), smem, stream, p, shared_tiles, (int)n_shared);
+      if (e != cudaSuccess) return (int)e;
+    }
+    return (int)launch(kernel, dim3((unsigned)n_own), dim3(kShThreads), smem, stream, p, own_tiles, 0);
+  };
+  return p.dv <= 128 ? run(shared_parts_kernel<T, 1>) : run(shared_parts_kernel<T, 2>);
+}
+
+template <typename T>
+static int launch_merge(const SharedParams& p, cudaStream_t stream) {
+  const long long pairs = (long long)p.n_rows * p.n_q_heads;
+  return (int)launch(shared_merge_kernel<T>, dim3((unsigned)((pairs + kMergeWarps - 1) / kMergeWarps)), dim3(kMergeWarps * 32), 0,
+                     stream, p);
+}
+
+}  // namespace tk
+
+// scratch: rows * n_q_heads * (n_shared + n_own) * (dv + 2) floats.
+TK_API int tk_attention_shared(const void* q, void* out, const void* k_cache, const void* v_cache, const int* group_start,
+                               const int* prefix_slot, const int* prefix_len, const int* positions, const int* req_slot,
+                               const int* block_table, const unsigned char* history, const float* sinks, float* scratch,
+                               int* err, int n_rows, int n_groups, int max_members, int n_q_heads, int n_kv_heads, int head_dim,
+                               int v_dim, int page_size, int max_pages, int num_pages, int max_slots, int history_ld,
+                               int window, int n_shared, int n_own, float scale, float softcap, int dtype,
+                               cudaStream_t stream) {
+  if (n_rows <= 0 || n_groups <= 0) return 0;
+  const long long parts = (long long)n_rows * n_q_heads * ((long long)n_shared + n_own);
+  if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads != 0 || head_dim < 1 || head_dim > 256 || v_dim < 1 || v_dim > 256 ||
+      page_size < 1 || max_members < 1 || n_shared < 0 || n_own < 1 || max_slots < 1 || max_pages < 1 ||
+      parts > 0x7fffffffLL || (history != nullptr && history_ld < 1)) {
+    return (int)cudaErrorInvalidValue;
+  }
+  tk::SharedParams p;
+  p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.group_start = group_start; p.prefix_slot = prefix_slot;
+  p.prefix_len = prefix_len; p.positions = positions; p.req_slot = req_slot; p.block_table = block_table; p.history = history;
+  p.sinks = sinks; p.err = err;
+  p.n_rows = n_rows; p.n_groups = n_groups; p.max_members = max_members; p.n_q_heads = n_q_heads; p.n_kv_heads = n_kv_heads;
+  p.d = head_dim; p.dv = v_dim; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages;
+  p.max_slots = max_slots; p.history_ld = history_ld; p.window = window;
+  p.n_shared = n_shared; p.n_own = n_own; p.n_parts = n_shared + n_own;
+  p.part_o = scratch;
+  p.part_ml = scratch + parts * v_dim;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.cap_log2 = softcap > 0.0f ? softcap * 1.4426950408889634f : 0.0f;
+  p.inv_cap = softcap > 0.0f ? scale / softcap : 0.0f;
+  const uintptr_t mask = dtype == tk::kF32 ? 15 : 7;
+  p.wide_k = head_dim % 4 == 0 && (((uintptr_t)q | (uintptr_t)k_cache) & mask) == 0;
+  p.wide_v = v_dim % 4 == 0 && ((uintptr_t)v_cache & mask) == 0;
+  if (dtype == tk::kF32) {
+    const int e = tk::launch_general<float>(p, stream);
+    return e != 0 ? e : tk::launch_merge<float>(p, stream);
+  }
+  if (dtype != tk::kBF16) return (int)cudaErrorInvalidValue;
+  const int e = tk::launch_general<__nv_bfloat16>(p, stream);
+  return e != 0 ? e : tk::launch_merge<__nv_bfloat16>(p, stream);
+}

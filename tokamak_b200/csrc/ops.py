@@ -220,6 +220,177 @@ def sample_slots(logits: torch.Tensor, records: torch.Tensor, row_slot: torch.Te
                                      err.data_ptr(), _stream()), "sample_slots")
 
 
+def _want_here(**tensors) -> None:
+    """Refuses tensors of a device other than the current one: the launch goes to the current device's stream."""
+    here = _raw_device()
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"{name} must be on the current CUDA device {here}, it is on {t.device}")
+
+
+BEAM_MAX = 64                     # beams of a group
+BEAM_MAX_CANDIDATES = 256
+_BEAM_MAX_ENTRIES = 16384         # beams * segments * candidates that the kernel which joins a group's segments takes
+_BEAM_TILE = 4096                 # logits that a block has in flight at a time
+BEAM_SEAT_LIMIT = 64              # seats of a group that reorder_slots moves between
+
+
+def beam_segments(device: torch.device, rows: int, beams: int, vocab: int, candidates: int) -> int:
+    """Segments that a row of logits is cut into: as many as fill the SMs with two blocks each, none shorter than a block's
+    tile, and no more than the joining kernel holds the candidates of."""
+    fill = 2 * sm_count(device) // max(1, rows)
+    return max(1, min(fill, -(-vocab // _BEAM_TILE), _BEAM_MAX_ENTRIES // (beams * candidates)))
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int, *, out: tuple | None = None
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The ``candidates`` best continuations of every group of beams, best first: ``(scores, parents, tokens)``, each
+    ``[groups, candidates]`` (float32, int32, int32).
+
+    ``logits`` are float32 ``[groups * beams, vocab]`` (rows may lie further apart), ``scores`` ``[groups, beams]`` the
+    beams' sums of log probabilities.  A continuation's score is its beam's plus the log softmax of its logit; scores are
+    compared in 64 bits and rounded once.  Equal ones: the larger logit of one beam first, then the lower beam, then the lower
+    token.  A beam with a score of -inf or NaN is not read; its continuations, with scores of -inf, come last, and so do
+    logits of -inf or NaN.  ``out``: tensors to write to."""
+    if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
+        raise KernelError("logits must be a float32 CUDA tensor [groups * beams, vocab] whose rows are contiguous")
+    _want(scores, torch.float32, "scores")
+    if scores.dim() != 2:
+        raise KernelError(f"scores must be [groups, beams], got shape {tuple(scores.shape)}")
+    groups, beams = scores.shape
+    rows, vocab = logits.shape
+    if rows != groups * beams:
+        raise KernelError(f"{rows} rows of logits for {groups} groups of {beams} beams")
+    if not 1 <= beams <= BEAM_MAX or vocab < 1:
+        raise KernelError(f"a group has 1 to {BEAM_MAX} beams over one token at least, got {beams} over {vocab}")
+    if not 1 <= candidates <= min(BEAM_MAX_CANDIDATES, beams * vocab):
+        raise KernelError(f"1 to {min(BEAM_MAX_CANDIDATES, beams * vocab)} candidates of a group can be asked for, got {candidates}")
+    if rows > SAMPLING_MAX_ROWS or vocab > SAMPLING_MAX_VOCAB:
+        raise KernelError(f"the selection takes up to {SAMPLING_MAX_ROWS} rows of up to {SAMPLING_MAX_VOCAB} logits, "
+                          f"got {rows} x {vocab}")
+    if rows > 1 and logits.stride(0) < vocab:
+        raise KernelError("rows of logits overlap")
+    shape = (groups, candidates)
+    if out is None:
+        out = (torch.empty(shape, dtype=torch.float32, device=logits.device),
+               torch.empty(shape, dtype=torch.int32, device=logits.device),
+               torch.empty(shape, dtype=torch.int32, device=logits.device))
+    for name, t, dtype in zip(("scores", "parents", "tokens"), out, (torch.float32, torch.int32, torch.int32)):
+        _want(t, dtype, "out " + name)
+        if t.shape != shape:
+            raise KernelError(f"out {name} must be {shape}, got {tuple(t.shape)}")
+    _want_here(logits=logits, scores=scores, out=out[0], parents=out[1], tokens=out[2])
+    if groups == 0:
+        return out
+    segments = beam_segments(logits.device, rows, beams, vocab, candidates)
+    scratch = torch.empty(rows * segments * (2 + candidates), dtype=torch.int64, device=logits.device)
+    _check(_lib().tk_beam_select(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, scores.data_ptr(),
+                                 scratch.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), groups, beams,
+                                 vocab, candidates, segments, _stream()), "beam_select")
+    return out
+
+
+def beam_advance(candidates: tuple, stop_tokens: torch.Tensor | None, slots: torch.Tensor, scores: torch.Tensor,
+                 parents: torch.Tensor, tokens: torch.Tensor, err: torch.Tensor, *, records: torch.Tensor | None = None,
+                 token_word: int = 7, history: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                 prefix_len: torch.Tensor | None = None, begin: bool = False) -> None:
+    """The beams that go on after :func:`beam_select`: of a group's candidates, in order, the first whose tokens are not in
+    ``stop_tokens`` (int32), as many as it has beams.
+
+    Written for every seat (``[groups, beams]``): the beam's new score, the seat that it goes on from and its token.  A beam
+    stays in its parent's seat unless a better one took it; the rest fill the other seats in order, so a seat that goes
+    on is never written by :func:`reorder_slots`.  A seat that is left over goes on from itself with a score of -inf and token 0.
+    ``records`` (int32 ``[slots, words]``): word ``token_word`` of the record of each seat's slot (``slots`` ``[groups,
+    beams]``) receives the token.  ``history`` (uint8 ``[slots, n]``): the place ``positions - prefix_len`` of each
+    seat's row receives the seat (see :class:`SharedPrefix`); call :func:`reorder_slots` afterwards.  ``begin``: the candidates
+    continue one row (a search that begins); every seat goes on from itself, and the history is left alone."""
+    for name, t, dtype in (("candidate scores", candidates[0], torch.float32), ("candidate parents", candidates[1], torch.int32),
+                           ("candidate tokens", candidates[2], torch.int32)):
+        _want(t, dtype, name)
+        if t.dim() != 2 or t.shape != candidates[0].shape:
+            raise KernelError("the candidates must be three tensors [groups, candidates]")
+    groups, k = candidates[0].shape
+    for name, t, dtype in (("slots", slots, torch.int32), ("scores", scores, torch.float32), ("parents", parents, torch.int32),
+                           ("tokens", tokens, torch.int32)):
+        _want(t, dtype, name)
+        if t.dim() != 2 or t.shape != slots.shape or t.shape[0] != groups:
+            raise KernelError(f"{name} must be [groups, beams] for {groups} groups, got {tuple(t.shape)}")
+    beams = slots.shape[1]
+    if not 1 <= beams <= BEAM_MAX or k < 1:
+        raise KernelError(f"a group has 1 to {BEAM_MAX} beams and a candidate at least, got {beams} and {k}")
+    _want(err, torch.int32, "err")
+    n_stop = 0
+    if stop_tokens is not None:
+        _want(stop_tokens, torch.int32, "stop_tokens")
+        n_stop = stop_tokens.numel()
+    max_slots, words, ld = 1 << 30, 0, 0
+    if records is not None:
+        _want(records, torch.int32, "records")
+        if records.dim() != 2 or not 0 <= token_word < records.shape[1]:
+            raise KernelError(f"records must be [slots, words] with a word {token_word}, got {tuple(records.shape)}")
+        max_slots, words = records.shape
+    if history is not None:
+        _want(history, torch.uint8, "history")
+        if history.dim() != 2 or (records is not None and history.shape[0] != max_slots):
+            raise KernelError("history must be [slots, n] for the slots of the records")
+        max_slots, ld = history.shape
+        if not begin:
+            if positions is None or prefix_len is None:
+                raise KernelError("a history needs the positions that the step wrote and prefix_len")
+            _want(positions, torch.int32, "positions"); _want(prefix_len, torch.int32, "prefix_len")
+            if positions.numel() < groups * beams or prefix_len.numel() < groups:
+                raise KernelError("positions or prefix_len is shorter than the batch")
+    _want_here(candidates=candidates[0], stop_tokens=stop_tokens, slots=slots, scores=scores, records=records,
+               history=history, err=err)
+    if groups == 0:
+        return
+    _check(_lib().tk_beam_advance(candidates[0].data_ptr(), candidates[1].data_ptr(), candidates[2].data_ptr(), _ptr(stop_tokens),
+                                  slots.data_ptr(), scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _ptr(records),
+                                  _ptr(history), _ptr(positions), _ptr(prefix_len), err.data_ptr(), groups, beams, k, n_stop,
+                                  max_slots, words, int(token_word), ld, int(begin), _stream()), "beam_advance")
+
+
+_REORDER_TENSORS = 24             # tensors of one launch
+
+
+def reorder_slots(records, slots: torch.Tensor, parents: torch.Tensor, err: torch.Tensor) -> None:
+    """``t[:, slots[g, i]] <- t[:, slots[g, parents[g, i]]]`` for all seats ``i`` of a group at once and in place, for every
+    tensor ``t`` ``[keys, slots, ...]`` of fixed-size records in ``records`` (any type): what a request's slot keeps on the
+    device follows the beam that goes on in it.
+
+    ``slots`` and ``parents`` are int32 ``[groups, seats]``; a slot belongs to one seat of one group.  A seat whose parent
+    is itself is not touched, whatever else is in the tensors is left as it is.  A parent outside the group or a slot outside
+    the tensors is reported through ``err`` and that seat stays as it is."""
+    _want(slots, torch.int32, "slots"); _want(parents, torch.int32, "parents"); _want(err, torch.int32, "err")
+    if slots.dim() != 2 or parents.shape != slots.shape:
+        raise KernelError(f"slots and parents must be [groups, seats], got {tuple(slots.shape)} and {tuple(parents.shape)}")
+    groups, seats = slots.shape
+    if not 1 <= seats <= BEAM_SEAT_LIMIT or groups > 65535:
+        raise KernelError(f"records move between 1 to {BEAM_SEAT_LIMIT} seats of up to 65535 groups, got {seats} of {groups}")
+    bases, sizes, keys, max_slots = [], [], [], None
+    here = _raw_device()
+    for t in records:
+        if not t.is_cuda or not t.is_contiguous() or t.dim() < 2:
+            raise KernelError("records must be contiguous CUDA tensors [keys, slots, ...]")
+        if max_slots is None:
+            max_slots = t.shape[1]
+        if t.shape[1] != max_slots or max_slots < 1:
+            raise KernelError("all records must have the same number of slots")
+        if t.get_device() != here:
+            raise KernelError(f"records must be on the current CUDA device {here}")
+        n = t.numel() * t.element_size()
+        if n:
+            bases.append(t.data_ptr()); keys.append(t.shape[0]); sizes.append(n // (t.shape[0] * max_slots))
+    _want_here(slots=slots, parents=parents, err=err)
+    if groups == 0:
+        return
+    for i in range(0, len(bases), _REORDER_TENSORS):
+        n = min(_REORDER_TENSORS, len(bases) - i)
+        _check(_lib().tk_reorder_slots((ctypes.c_void_p * n)(*bases[i:i + n]), (ctypes.c_longlong * n)(*sizes[i:i + n]),
+                                       (ctypes.c_int * n)(*keys[i:i + n]), n, slots.data_ptr(), parents.data_ptr(),
+                                       err.data_ptr(), groups, seats, max_slots, _stream()), "reorder_slots")
+
+
 def wait_probe(limit: int, err: torch.Tensor) -> None:
     """Test aid: one block waits on a barrier that nobody arrives at, gives up after ``limit``
     polls and reports it through the error word exactly as the tcgen05 kernels would."""
@@ -1788,6 +1959,101 @@ def attention_prefill_tc(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tens
                                           float(scale), float(softcap or 0.0), _ptr(sinks), int(chunk or 0),
                                           _ptr(slopes), _ptr(dist_bias), _want_dist_bias(dist_bias, hq), _stream()),
            "attention_prefill_tc")
+
+
+@dataclass
+class SharedPrefix:
+    """What the requests of a step of single next tokens share, for :func:`attention_shared`.
+
+    The rows ``group_start[g] .. group_start[g + 1] - 1`` (int32 ``[groups + 1]``) share the positions below
+    ``prefix_len[g]``, which lie in the pages of the block table's row ``prefix_slot[g]``.  ``history`` (uint8 ``[slots, n]``):
+    position ``prefix_len + i`` of the request in slot ``s`` was written by the member ``history[s, i]`` of its group
+    and lies in that member's pages; without it every request reads its own.  The position of a row itself is its own.
+    ``max_members``, ``max_prefix`` and ``max_own`` bound the members of a group, ``prefix_len``, and the positions behind it
+    (the new token among them): the work is planned for them."""
+
+    group_start: torch.Tensor
+    prefix_slot: torch.Tensor
+    prefix_len: torch.Tensor
+    max_members: int
+    max_prefix: int
+    max_own: int
+    history: torch.Tensor | None = None
+
+
+def shared_splits(device: torch.device, groups: int, rows: int, n_q_heads: int, n_kv_heads: int, shared: SharedPrefix,
+                  window: int | None) -> tuple[int, int]:
+    """Parts that the shared and the other positions are cut into: enough blocks for two an SM, none with less than 64 keys."""
+    sms = sm_count(device)
+    per = n_q_heads // n_kv_heads
+    keys = min(shared.max_prefix, window or shared.max_prefix)
+    blocks = groups * n_kv_heads * -(-shared.max_members * per // 32)
+    n_shared = max(1, min(2 * sms // max(1, blocks), -(-keys // 64))) if keys > 0 else 0
+    own = min(shared.max_own, window or shared.max_own)
+    n_own = max(1, min(2 * sms // max(1, rows * n_kv_heads), -(-own // 64)))
+    return n_shared, n_own
+
+
+def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, shared: SharedPrefix,
+                     positions: torch.Tensor, req_slot: torch.Tensor, block_table: torch.Tensor, err: torch.Tensor, *,
+                     scale: float, window: int | None = None, softcap: float | None = None,
+                     sinks: torch.Tensor | None = None) -> None:
+    """Paged attention of one token per request over keys that groups of requests share.
+
+    Row ``r`` of ``q`` ``[rows, Hq, d]`` is the token at ``positions[r]`` of the request in slot ``req_slot[r]``; it sees the
+    positions up to its own (the last ``window`` of them), the shared ones read once for all members of its group.  Caches
+    ``[pages, Hkv, page, d]`` (values ``dv``) and ``block_table`` ``[slots, pages]`` as in the other attention kernels, float32
+    or bfloat16; ``softcap`` and ``sinks`` as in :func:`attention_plain`.  Cached keys and values must be finite wherever
+    a member of the group sees them."""
+    _want(q, None, "q"); _want(out, q.dtype, "out"); _want(k_cache, q.dtype, "k_cache"); _want(v_cache, q.dtype, "v_cache")
+    dtype = dtype_code(q.dtype)
+    _want(positions, torch.int32, "positions"); _want(req_slot, torch.int32, "req_slot")
+    _want(block_table, torch.int32, "block_table"); _want(err, torch.int32, "err")
+    for name in ("group_start", "prefix_slot", "prefix_len"):
+        _want(getattr(shared, name), torch.int32, name)
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4 or block_table.dim() != 2:
+        raise KernelError("q must be [rows, Hq, d], the caches [pages, Hkv, page, d], the block table [slots, pages]")
+    rows, hq, d = q.shape
+    num_pages, hkv, page_size, dk = k_cache.shape
+    dv = v_cache.shape[3]
+    groups = shared.prefix_len.numel()
+    if dk != d or tuple(v_cache.shape[:3]) != (num_pages, hkv, page_size) or tuple(out.shape) != (rows, hq, dv):
+        raise KernelError(f"queries {tuple(q.shape)}, caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} and output "
+                          f"{tuple(out.shape)} do not fit")
+    if hkv < 1 or hq % hkv or d > 256 or dv > 256:
+        raise KernelError(f"the shared-prefix attention takes query heads that are a multiple of the key heads, of up to 256 "
+                          f"elements; got {hq}/{hkv} of {d} and {dv}")
+    if positions.numel() < rows or req_slot.numel() < rows:
+        raise KernelError("positions or req_slot is shorter than the batch")
+    if shared.group_start.numel() != groups + 1 or shared.prefix_slot.numel() != groups:
+        raise KernelError("group_start must have one entry more than prefix_len, prefix_slot as many")
+    if rows and (groups < 1 or shared.max_members < 1 or shared.max_prefix < 0 or shared.max_own < 1):
+        raise KernelError("a step needs a group, a member, and an own position at least")
+    if window is not None and window < 1:
+        raise KernelError(f"a window of {window} positions is none")
+    history, ld = shared.history, 0
+    if history is not None:
+        _want(history, torch.uint8, "history")
+        if history.dim() != 2 or history.shape[0] != block_table.shape[0]:
+            raise KernelError("history must be [slots, n] for the slots of the block table")
+        if shared.max_members > 256:
+            raise KernelError(f"a history names up to 256 members of a group, got {shared.max_members}")
+        ld = history.shape[1]
+    _want_sinks(sinks, hq)
+    _want_here(q=q, out=out, k_cache=k_cache, v_cache=v_cache, positions=positions, req_slot=req_slot, block_table=block_table,
+               err=err, group_start=shared.group_start, prefix_slot=shared.prefix_slot, prefix_len=shared.prefix_len,
+               history=history, sinks=sinks)
+    if rows == 0:
+        return
+    n_shared, n_own = shared_splits(q.device, groups, rows, hq, hkv, shared, window)
+    scratch = torch.empty(rows * hq * (n_shared + n_own) * (dv + 2), dtype=torch.float32, device=q.device)
+    _check(_lib().tk_attention_shared(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                      shared.group_start.data_ptr(), shared.prefix_slot.data_ptr(), shared.prefix_len.data_ptr(),
+                                      positions.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), _ptr(history), _ptr(sinks),
+                                      scratch.data_ptr(), err.data_ptr(), rows, groups, shared.max_members, hq, hkv, d, dv,
+                                      page_size, block_table.shape[1], num_pages, block_table.shape[0], ld, int(window or 0),
+                                      n_shared, n_own, float(scale), float(softcap or 0.0), dtype, _stream()),
+           "attention_shared")
 
 
 def sm_count(device: torch.device) -> int:
