@@ -511,6 +511,15 @@ def test_shared_attention_long(dtype):
     c.check()
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("members", [[8], [9], [16, 3], [20, 17, 1], [33]])
+def test_shared_attention_of_many_query_heads(members, dtype, d):
+    """More (query head, member) pairs over a key head than a tile of rows, or two, hold."""
+    c = Shared(members, [150, 70, 200][:len(members)], 21, hq=16, hkv=1, d=d, dtype=dtype, history=True, seed=14).device()
+    c.call()
+    c.check()
+
+
 def test_shared_attention_at_addresses_on_any_boundary():
     for dtype in (torch.float32, torch.bfloat16):
         c = Shared([3], [70], 20, d=64, dtype=dtype, seed=13).device()

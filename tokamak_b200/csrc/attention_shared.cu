@@ -1,108 +1,8 @@
-// Paged attention of single next tokens whose requests share a prefix (a system prompt, the beams of one search).
-//
-// Rows (one token each) come in groups: the rows group_start[g] .. group_start[g + 1] - 1 share the positions
-// [0, prefix_len[g]), which lie in the pages of block-table row prefix_slot[g].  A position behind them lies in the
-// pages of the row's own request, or, with a history, in those of the member of the group that wrote it: the beams of a search
-// keep their keys where they were written, and what a beam inherits is a list of writers (history[slot][n] is the
-// member that wrote position prefix_len + n; the row's own position is always its own).  A row at position pos sees
-// [max(0, pos - window + 1), pos].
-//
-// The query heads of all members over one key/value head are the rows of one matrix product over the shared keys, so
-// these are read once for the group instead of once for every member: out = sum_j softmax(s)_j v_j is taken apart into the
-// part over the shared positions and the part over the others, each with its maximum m, its sum l of 2^(s - m) and its
-// unnormalised output o, all in float32, and the parts are added up as sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
-//
-// This file: the general kernel (float32 or bfloat16, any head size up to 256) for both parts, and the one that adds
-// parts up.
-#include "mma_utils.cuh"
+// Attention over shared prefixes: the general kernel (float32 or bfloat16, any head size up to 256) for both parts, the
+// one that adds parts up, and the entry point.  attention_shared.cuh has the definition.
+#include "attention_shared.cuh"
 
 namespace tk {
-
-struct SharedParams {
-  const void* q;                // [rows, n_q_heads, d]
-  void* out;                    // [rows, n_q_heads, dv]
-  const void* k_cache;          // [num_pages, n_kv_heads, page_size, d]
-  const void* v_cache;          // [num_pages, n_kv_heads, page_size, dv]
-  const int* group_start;       // [n_groups + 1]
-  const int* prefix_slot;       // [n_groups]
-  const int* prefix_len;        // [n_groups]
-  const int* positions;         // [rows]
-  const int* req_slot;          // [rows]
-  const int* block_table;       // [max_slots, max_pages]
-  const unsigned char* history; // [max_slots, history_ld] or null
-  const float* sinks;           // [n_q_heads] or null
-  float* part_o;                // [rows, n_q_heads, n_parts, dv]
-  float* part_ml;               // [rows, n_q_heads, n_parts, 2]
-  int* err;
-  int n_rows, n_groups, max_members, n_q_heads, n_kv_heads, d, dv, page_size, max_pages, num_pages, max_slots, history_ld, window;
-  int n_shared, n_own, n_parts; // parts of the shared and of the other positions; n_parts = n_shared + n_own
-  int wide_k, wide_v;           // rows of queries and keys, of values, can be read four elements at a time
-  float scale_log2, cap_log2, inv_cap;
-};
-
-// The group that holds a row: the last one that starts at or before it.
-__device__ __forceinline__ int group_of_row(const SharedParams& p, int row) {
-  int lo = 0, hi = p.n_groups - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.group_start[mid] <= row) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
-
-// Rows of group g, cut to what exists.
-__device__ __forceinline__ int2 group_rows(const SharedParams& p, int g) {
-  const int a = max(0, min(p.n_rows, p.group_start[g]));
-  const int b = max(a, min(p.n_rows, p.group_start[g + 1]));
-  return make_int2(a, min(b, a + p.max_members));
-}
-
-__device__ __forceinline__ int checked_slot(const SharedParams& p, int slot, int row) {
-  if (slot >= 0 && slot < p.max_slots) return slot;
-  set_error(p.err, kErrRequest, row, slot, p.max_slots);
-  return -1;
-}
-
-// Place of a position in the pools: (page * n_kv_heads + head) * page_size + offset, -1 for one that has no page.
-__device__ __forceinline__ long long pool_row(const SharedParams& p, int slot, int pos, int hkv, int row) {
-  const int pidx = pos / p.page_size;
-  const int page = (slot >= 0 && pidx < p.max_pages) ? p.block_table[(size_t)slot * p.max_pages + pidx] : -1;
-  if (page < 0 || page >= p.num_pages) {
-    if (slot >= 0) set_error(p.err, kErrPage, row, pidx, page);
-    return -1;
-  }
-  return ((long long)page * p.n_kv_heads + hkv) * p.page_size + pos % p.page_size;
-}
-
-// The slot that holds position `pos` (behind the shared ones) of row `row`.
-__device__ __forceinline__ int writer_slot(const SharedParams& p, int row, int slot, int pos, int own_pos, int prefix, int2 rows) {
-  if (p.history == nullptr || pos == own_pos || slot < 0) return slot;
-  const int n = pos - prefix;
-  if (n >= p.history_ld) { set_error(p.err, kErrPosition, row, pos, p.history_ld); return -1; }
-  const int member = p.history[(size_t)slot * p.history_ld + n];
-  if (member >= rows.y - rows.x) { set_error(p.err, kErrRequest, row, member, rows.y - rows.x); return -1; }
-  return checked_slot(p, p.req_slot[rows.x + member], row);
-}
-
-// Whether the row belongs to a group as it should; where not, its shared parts are marked as empty here (head >= 0: for that
-// head), since no block of the shared positions does it, and an error is set.
-__device__ __forceinline__ bool row_has_group(const SharedParams& p, int row, int2 rows, int prefix, int head) {
-  if (row >= rows.x && row < rows.y && (p.n_shared > 0 || prefix == 0)) return true;
-  set_error(p.err, kErrRequest, row, p.max_members, prefix);
-  if (head >= 0) {
-    float* ml = p.part_ml + 2 * ((size_t)row * p.n_q_heads + head) * p.n_parts;
-    for (int i = 0; i < p.n_shared; ++i) { ml[2 * i] = -INFINITY; ml[2 * i + 1] = 0.0f; }
-  }
-  return false;
-}
-
-// What a row sees: [lo, pos]; bad positions see nothing.
-struct RowSpan { int pos, lo; };
-__device__ __forceinline__ RowSpan row_span(const SharedParams& p, int row) {
-  const int pos = p.positions[row];
-  if (pos < 0) { set_error(p.err, kErrPosition, row, pos, 0); return {-1, 0}; }
-  return {pos, first_visible(pos, p.window, 0)};
-}
 
 // ---- general kernel -----------------------------------------------------------------------------------------------
 //
@@ -324,27 +224,42 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_merge_kernel(SharedPa
   const long long pair = (long long)blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
   if (pair >= (long long)p.n_rows * p.n_q_heads) return;
   const int head = (int)(pair % p.n_q_heads);
-  const float* ml = p.part_ml + 2 * pair * p.n_parts;
-  float m_all = -INFINITY;
-  for (int i = lane; i < p.n_parts; i += 32) m_all = fmaxf(m_all, __ldcg(ml + 2 * i));
-  m_all = warp_max(m_all);
-  float l_all = 0.0f;
-  for (int i = lane; i < p.n_parts; i += 32) {
-    const float l = __ldcg(ml + 2 * i + 1);
-    if (l > 0.0f) l_all += l * exp2f(__ldcg(ml + 2 * i) - m_all);
-  }
-  l_all = warp_sum(l_all);
-  const float inv = l_all > 0.0f ? 1.0f / (l_all + sink_term_log2(p.sinks, head, m_all)) : 0.0f;
-  T* out = (T*)p.out + pair * p.dv;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + pair * p.n_parts;
   const float* o = p.part_o + (size_t)pair * p.n_parts * p.dv;
-  for (int c0 = 0; c0 < p.dv; c0 += 32) {
-    const int c = c0 + lane;
-    float acc = 0.0f;
-    for (int i = 0; i < p.n_parts; ++i) {
-      const float l = __ldcg(ml + 2 * i + 1);
-      if (l > 0.0f && c < p.dv) acc += __ldcg(o + (size_t)i * p.dv + c) * exp2f(__ldcg(ml + 2 * i) - m_all);
+  float2 mine = lane < p.n_parts ? __ldcg(ml + lane) : make_float2(-INFINITY, 0.0f);
+  float m_all = mine.x;
+  for (int i = lane + 32; i < p.n_parts; i += 32) m_all = fmaxf(m_all, __ldcg(ml + i).x);
+  m_all = warp_max(m_all);
+  const bool wide = p.dv % 4 == 0;
+  T* out = (T*)p.out + pair * p.dv;
+  for (int c0 = 0; c0 < p.dv; c0 += 128) {
+    const int c = c0 + 4 * lane;
+    float l_all = 0.0f;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = 0; i0 < p.n_parts; i0 += 32) {
+      if (i0 > 0 || c0 > 0) mine = i0 + lane < p.n_parts ? __ldcg(ml + i0 + lane) : make_float2(-INFINITY, 0.0f);
+      const float f = mine.y > 0.0f ? exp2f(mine.x - m_all) : 0.0f;
+      l_all += f * mine.y;
+      const int n = min(32, p.n_parts - i0);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float w = __shfl_sync(0xffffffffu, f, i);
+        if (w == 0.0f || c >= p.dv) continue;        // an empty part has no output that is anything
+        const float* src = o + (size_t)(i0 + i) * p.dv + c;
+        if (wide) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+          acc[0] += v.x * w; acc[1] += v.y * w; acc[2] += v.z * w; acc[3] += v.w * w;
+        } else {
+          for (int e = 0; e < 4 && c + e < p.dv; ++e) acc[e] += __ldcg(src + e) * w;
+        }
+      }
     }
-    if (c < p.dv) out[c] = from_f32<T>(acc * inv);
+    l_all = warp_sum(l_all);
+    const float inv = l_all > 0.0f ? 1.0f / (l_all + sink_term_log2(p.sinks, head, m_all)) : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (c + e < p.dv) out[c + e] = from_f32<T>(acc[e] * inv);
+    }
   }
 }
 
@@ -378,7 +293,14 @@ static int launch_merge(const SharedParams& p, cudaStream_t stream) {
 
 }  // namespace tk
 
-// scratch: rows * n_q_heads * (n_shared + n_own) * (dv + 2) floats.
+// Whether the kernels of attention_shared_tc.cu take a shape (addresses on 16 bytes besides).
+TK_API int tk_attention_shared_tc_takes(int n_q_heads, int n_kv_heads, int head_dim, int v_dim, int page_size) {
+  tk::SharedParams p = {};
+  p.n_q_heads = n_q_heads; p.n_kv_heads = n_kv_heads; p.d = head_dim; p.dv = v_dim; p.page_size = page_size;
+  return tk::shared_tc_takes(p);
+}
+
+// scratch: rows * n_q_heads * (n_shared + n_own) * (dv + 2) floats on 16 bytes, with an odd v_dim one more.
 TK_API int tk_attention_shared(const void* q, void* out, const void* k_cache, const void* v_cache, const int* group_start,
                                const int* prefix_slot, const int* prefix_len, const int* positions, const int* req_slot,
                                const int* block_table, const unsigned char* history, const float* sinks, float* scratch,
@@ -402,7 +324,7 @@ TK_API int tk_attention_shared(const void* q, void* out, const void* k_cache, co
   p.max_slots = max_slots; p.history_ld = history_ld; p.window = window;
   p.n_shared = n_shared; p.n_own = n_own; p.n_parts = n_shared + n_own;
   p.part_o = scratch;
-  p.part_ml = scratch + parts * v_dim;
+  p.part_ml = scratch + (parts * v_dim + 1) / 2 * 2;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.cap_log2 = softcap > 0.0f ? softcap * 1.4426950408889634f : 0.0f;
   p.inv_cap = softcap > 0.0f ? scale / softcap : 0.0f;
@@ -414,6 +336,6 @@ TK_API int tk_attention_shared(const void* q, void* out, const void* k_cache, co
     return e != 0 ? e : tk::launch_merge<float>(p, stream);
   }
   if (dtype != tk::kBF16) return (int)cudaErrorInvalidValue;
-  const int e = tk::launch_general<__nv_bfloat16>(p, stream);
+  const int e = tk::shared_tc_takes(p) ? tk::launch_shared_tc(p, stream) : tk::launch_general<__nv_bfloat16>(p, stream);
   return e != 0 ? e : tk::launch_merge<__nv_bfloat16>(p, stream);
 }

@@ -8,8 +8,10 @@ is no CPU path: a tensor that is not on a CUDA device is an error.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from dataclasses import dataclass
+from functools import lru_cache
 
 import numpy as np
 import torch
@@ -1981,16 +1983,29 @@ class SharedPrefix:
     history: torch.Tensor | None = None
 
 
+@lru_cache(maxsize=None)
+def shared_tc_takes(n_q_heads: int, n_kv_heads: int, head_dim: int, v_dim: int, page_size: int) -> bool:
+    """Shapes of the tensor-core kernels of the shared-prefix attention (bfloat16); everything else goes to the general one."""
+    return bool(library().tk_attention_shared_tc_takes(n_q_heads, n_kv_heads, head_dim, v_dim, page_size))
+
+
 def shared_splits(device: torch.device, groups: int, rows: int, n_q_heads: int, n_kv_heads: int, shared: SharedPrefix,
-                  window: int | None) -> tuple[int, int]:
-    """Parts that the shared and the other positions are cut into: enough blocks for two an SM, none with less than 64 keys."""
+                  window: int | None, tensor_cores: bool) -> tuple[int, int]:
+    """Parts that the shared and the other positions are cut into.  The tensor-core kernel of the shared ones has a block per
+    SM and 128 or 256 (query head, member) pairs in each; all other blocks are small and several to an SM."""
     sms = sm_count(device)
     per = n_q_heads // n_kv_heads
     keys = min(shared.max_prefix, window or shared.max_prefix)
-    blocks = groups * n_kv_heads * -(-shared.max_members * per // 32)
-    n_shared = max(1, min(2 * sms // max(1, blocks), -(-keys // 64))) if keys > 0 else 0
+    if tensor_cores:
+        tile = 128 // per
+        tile *= 2 if shared.max_members > tile else 1
+        fill, least = sms, 128
+    else:
+        tile, fill, least = 32 / per, 2 * sms, 64
+    blocks = groups * n_kv_heads * math.ceil(shared.max_members / tile)
+    n_shared = max(1, min(fill // blocks, -(-keys // least))) if keys > 0 else 0
     own = min(shared.max_own, window or shared.max_own)
-    n_own = max(1, min(2 * sms // max(1, rows * n_kv_heads), -(-own // 64)))
+    n_own = max(1, min(2 * sms // max(1, rows * n_kv_heads), -(-own // least)))
     return n_shared, n_own
 
 
@@ -2045,8 +2060,9 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
                history=history, sinks=sinks)
     if rows == 0:
         return
-    n_shared, n_own = shared_splits(q.device, groups, rows, hq, hkv, shared, window)
-    scratch = torch.empty(rows * hq * (n_shared + n_own) * (dv + 2), dtype=torch.float32, device=q.device)
+    tensor_cores = dtype == 1 and shared_tc_takes(hq, hkv, d, dv, page_size)
+    n_shared, n_own = shared_splits(q.device, groups, rows, hq, hkv, shared, window, tensor_cores)
+    scratch = torch.empty(rows * hq * (n_shared + n_own) * (dv + 2) + 1, dtype=torch.float32, device=q.device)
     _check(_lib().tk_attention_shared(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                       shared.group_start.data_ptr(), shared.prefix_slot.data_ptr(), shared.prefix_len.data_ptr(),
                                       positions.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), _ptr(history), _ptr(sinks),
