@@ -1,10 +1,11 @@
 """tokamak_b200: a single-GPU inference engine for the Qwen3 dense decoder on NVIDIA B200."""
 
+from .sampling.beam import BeamSearchParams
 from .sampling.params import SamplingParams
 
 __version__ = "0.1.0"
 
-__all__ = ["LLM", "RequestOutput", "SamplingParams", "__version__"]
+__all__ = ["LLM", "BeamHypothesis", "BeamSearchOutput", "BeamSearchParams", "RequestOutput", "SamplingParams", "__version__"]
 
 
 def __getattr__(name):
@@ -12,7 +13,7 @@ def __getattr__(name):
     if name == "LLM":
         from .engine.llm import LLM
         return LLM
-    if name == "RequestOutput":
-        from .engine.outputs import RequestOutput
-        return RequestOutput
+    if name in ("BeamHypothesis", "BeamSearchOutput", "RequestOutput"):
+        from .engine import outputs
+        return getattr(outputs, name)
     raise AttributeError(name)

@@ -137,18 +137,18 @@ class DeviceCache:
 
     # ---- the engine's records ----------------------------------------------------------------
     def write_record(self, slot: int, *, temperature: float, top_k: int, top_p: float, seed: int,
-                     counter: int = 0, fresh: bool = True) -> None:
+                     counter: int = 0, fresh: bool = True, computed: int = 0, last_token: int = -1) -> None:
         """Queue a slot's record for the next step's updates.  ``fresh`` (a newly admitted request)
-        also puts the position to 0 and the last token to none; without it only the sampling
-        parameters, the seed and the counter are replaced."""
+        also puts the position to ``computed`` (0, but for a request that was forked off another) and the last token
+        to ``last_token`` (none); without it only the sampling parameters, the seed and the counter are replaced."""
         import struct
         if not 0 <= slot < min(self.manager.max_slots, 1 << 16):
             raise ValueError(f"slot {slot} is outside the records")
         bits = lambda x: struct.unpack("<i", struct.pack("<f", float(x)))[0]
         wrap = lambda x: ((int(x) & 0xFFFFFFFF) ^ 0x80000000) - 0x80000000      # as a signed word
         seed &= 0x7FFFFFFFFFFFFFFF
-        words = [0, int(counter), wrap(seed), wrap(seed >> 32), bits(temperature), int(top_k),
-                 bits(top_p), -1]
+        words = [int(computed), int(counter), wrap(seed), wrap(seed >> 32), bits(temperature), int(top_k),
+                 bits(top_p), int(last_token)]
         mask = 0xFF if fresh else 0x7E
         old = self._record_writes.get(slot)
         if old is not None and not fresh:

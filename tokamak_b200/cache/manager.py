@@ -179,6 +179,16 @@ class KVGroup:
         entry.table.extend(pages)
         return [(start + i, page) for i, page in enumerate(pages)]
 
+    def fork(self, parent_id: Hashable, child_id: Hashable, length: int) -> None:
+        """A request that goes on behind the first ``length`` positions of another: it holds none of their pages (whoever
+        reads them goes by the parent's table), and its own begin with the page that position ``length`` falls into."""
+        if child_id in self._requests:
+            raise ValueError(f"request {child_id!r} holds pages already")
+        if self.pages_for(length) > len(self.table(parent_id)):
+            raise ValueError(f"request {parent_id!r} does not hold {length} positions")
+        below = length // self.page_size
+        self._requests[child_id] = _RequestPages(table=[-1] * below, released=below)
+
     def release_passed(self, req_id: Hashable, next_position: int) -> int:
         """Give back the pages that no query at ``next_position`` or later can see.
 
@@ -255,6 +265,20 @@ class CacheManager:
         self._slot_of[req_id] = slot
         self._length[req_id] = 0
         self.fresh_slots.add(slot)
+        return slot
+
+    def fork(self, parent_id: Hashable, child_id: Hashable) -> int:
+        """Give ``child_id`` a slot in which it goes on behind everything that ``parent_id`` has in the cache.  The child
+        reads the parent's pages, so the parent must stay live and as long as it is until the child is freed; state
+        records are not cleared: the caller copies the parent's."""
+        if parent_id not in self._slot_of:
+            raise KeyError(f"request {parent_id!r} has no slot; nothing can be forked off it")
+        length = self._length[parent_id]
+        slot = self.admit(child_id)
+        for g in self.kv_groups:
+            g.fork(parent_id, child_id, length)
+        self._length[child_id] = length
+        self.fresh_slots.discard(slot)
         return slot
 
     def length(self, req_id: Hashable) -> int:

@@ -30,6 +30,10 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--top-k", type=int, default=0)
     ap.add_argument("--seed", type=int, default=None, help="sampling seed (and seed of --write-random)")
     ap.add_argument("--ignore-eos", action="store_true")
+    ap.add_argument("--beam-width", type=int, default=0,
+                    help="search over this many beams instead of sampling and print the hypotheses, best first")
+    ap.add_argument("--length-penalty", type=float, default=1.0, help="with --beam-width: hypotheses are ranked by "
+                    "log probability over length to this power")
     ap.add_argument("--dtype", default="auto", choices=["auto", "bfloat16", "float32"])
     ap.add_argument("--max-seq-len", type=int, default=None)
     ap.add_argument("--block-size", type=int, default=16)
@@ -68,10 +72,14 @@ def main(argv: list[str] | None = None) -> int:
     if not args.model:
         raise SystemExit("--model is required")
 
-    from . import LLM, SamplingParams
+    from . import LLM, BeamSearchParams, SamplingParams
 
+    search = None
+    if args.beam_width:
+        search = BeamSearchParams(beam_width=args.beam_width, max_new_tokens=args.max_new_tokens,
+                                  length_penalty=args.length_penalty, ignore_eos=args.ignore_eos)
     llm = LLM(args.model, dtype=args.dtype, max_seq_len=args.max_seq_len, block_size=args.block_size,
-              kv_pool_tokens=args.kv_pool_tokens, max_batch_size=args.max_batch_size,
+              kv_pool_tokens=args.kv_pool_tokens, max_batch_size=max(args.max_batch_size, args.beam_width + 1),
               gpu_memory_utilization=args.gpu_memory_utilization,
               max_num_batched_tokens=args.max_num_batched_tokens, prefill_chunk=args.prefill_chunk,
               attention_policy=args.attention_policy, kv_watermark=args.kv_watermark,
@@ -86,7 +94,7 @@ def main(argv: list[str] | None = None) -> int:
             import torch
             gen = torch.Generator().manual_seed(args.seed or 0)
             ids = torch.randint(0, llm.model_config.vocab_size, (args.prompt_len,), generator=gen).tolist()
-        outputs = llm.generate(prompt_token_ids=[ids], sampling_params=params)
+        prompts = {"prompt_token_ids": [ids]}
         shown = f"{len(ids)} token ids"
     else:
         tok = llm.tokenizer
@@ -96,12 +104,19 @@ def main(argv: list[str] | None = None) -> int:
                                            add_generation_prompt=True, enable_thinking=False)
         except Exception:
             text = args.prompt
-        outputs = llm.generate(text, params)
+        prompts = {"prompts": text}
         shown = args.prompt
-    out = outputs[0]
+    written = lambda o: o.output_text if o.output_text else " ".join(str(t) for t in o.output_token_ids)
+    if search is not None:
+        found = llm.beam_search(params=search, **prompts)[0].hypotheses
+        print(f"\n[prompt]\n{shown}\n")
+        for i, h in enumerate(found):
+            print(f"[hypothesis {i} ({h.finish_reason.value}), score {h.score:.4f}]\n{written(h)}")
+        return 0
+    out = llm.generate(sampling_params=params, **prompts)[0]
     print(f"\n[prompt]\n{shown}\n")
     print(f"[completion ({out.finish_reason.value})]")
-    print(out.output_text if out.output_text else " ".join(str(t) for t in out.output_token_ids))
+    print(written(out))
     return 0
 
 

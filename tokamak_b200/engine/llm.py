@@ -17,13 +17,14 @@ from typing import Sequence as AbcSequence
 
 import torch
 
+from ..sampling.beam import BeamSearchParams
 from ..sampling.params import SamplingParams
 from .core import EngineCore
-from .outputs import RequestOutput
+from .outputs import BeamHypothesis, BeamSearchOutput, RequestOutput
 from dataclasses import dataclass
 
 from .scheduler import Scheduler, StepPlan
-from .sequence import Sequence
+from .sequence import FinishReason, Sequence
 from .step import PendingStep, SamplingRow, StepEntry
 
 logger = logging.getLogger(__name__)
@@ -136,6 +137,7 @@ class LLM:
         self.model = self.core.model
         self._tokenizer = None
         self.last_stats: dict = {}
+        self._beam_runner: tuple | None = None
         # A debugging aid: with plain_steps every step is laid out by the host (tokens included),
         # none is launched ahead of the one before it and none is replayed from a CUDA graph.  The
         # tokens must not depend on it.
@@ -248,6 +250,74 @@ class LLM:
         stats["pages_free"] = [g.num_free for g in self.cache_manager.kv_groups]
         self.last_stats = stats
         return [self._result_of(seq, texts[seq.seq_id] if texts else None) for seq in sequences]
+
+    def beam_search(self, prompts: str | AbcSequence[str] | None = None, params: BeamSearchParams | None = None, *,
+                    prompt_token_ids: AbcSequence[AbcSequence[int]] | None = None) -> list[BeamSearchOutput]:
+        """The best continuations of each prompt by a search over beams; one ``BeamSearchOutput`` per prompt, in input order.
+
+        Exactly one of ``prompts`` and ``prompt_token_ids`` is given.  A search takes ``beam_width + 1`` of the engine's
+        ``max_batch_size`` slots and the pages of its prompt and of every beam's continuation at its longest; searches that do
+        not fit side by side run one after the other.  Refused for models with attention that cannot read shared keys
+        and for more EOS tokens than there are candidates for."""
+        from .beam import STOPS_MAX, BeamRunner, Search, refuses_search
+        params = params or BeamSearchParams()
+        texts, token_lists = self._token_lists(prompts, prompt_token_ids)
+        why = refuses_search(self.model)
+        if why is not None:
+            raise ValueError(f"beam_search is not available for this model: {why}")
+        width, slots = params.beam_width, self.cache_manager.max_slots
+        if width + 1 > slots:
+            raise ValueError(f"a search of {width} beams takes {width + 1} slots, the engine has {slots}: raise max_batch_size")
+        stops = () if params.ignore_eos else tuple(self.model_config.eos_token_ids)
+        if len(stops) > STOPS_MAX:
+            raise ValueError(f"beam_search takes up to {STOPS_MAX} EOS tokens, the model has {len(stops)}")
+        searches, pages = [], []
+        for i, ids in enumerate(token_lists):
+            if not ids:
+                raise ValueError("a prompt needs at least one token")
+            self._check_request(Sequence(seq_id=i, prompt_token_ids=ids, sampling_params=SamplingParams(max_new_tokens=params.max_new_tokens)))
+            budget = min(params.max_new_tokens, self.max_seq_len - len(ids))
+            need = [g.pages_for(len(ids)) + width * (g.pages_for(len(ids) + budget) - len(ids) // g.page_size)
+                    for g in self.cache_manager.kv_groups]
+            for g, n in zip(self.cache_manager.kv_groups, need):
+                if n > g.num_pages:
+                    raise ValueError(f"a search of {width} beams over this prompt needs {n} cache pages and the pool has "
+                                     f"{g.num_pages}: raise kv_pool_tokens")
+            searches.append(Search(i, ids, budget))
+            pages.append(need)
+        if not searches:
+            return []
+        waves, left = [], []
+        for s, need in zip(searches, pages):
+            fits = waves and len(waves[-1]) < slots // (width + 1) and all(a >= b for a, b in zip(left, need))
+            if not fits:
+                waves.append([])
+                left = [g.num_pages for g in self.cache_manager.kv_groups]
+            waves[-1].append(s)
+            left = [a - b for a, b in zip(left, need)]
+        shape = (params.beam_width, stops, max(len(wave) for wave in waves), max(s.budget for s in searches))
+        if self._beam_runner is None or self._beam_runner[0] != shape:
+            self._beam_runner = (shape, BeamRunner(self.core.step, *shape))      # kept with the graphs it has captured
+        runner = self._beam_runner[1]
+        runner.start(params, min(self.max_num_batched_tokens, self.core.max_step_tokens))
+        graphs, self.core.step.use_graphs = self.core.step.use_graphs, self.core.step.use_graphs and not self.plain_steps
+        replays = self.core.step.graph_replays
+        try:
+            for wave in waves:
+                runner.run(wave)
+        finally:
+            self.core.step.use_graphs = graphs
+        self.last_stats = {"steps": runner.steps, "waves": len(waves), "graph_replays": self.core.step.graph_replays - replays,
+                           "pages_free": [g.num_free for g in self.cache_manager.kv_groups]}
+        decode = self.tokenizer.decode if self._has_tokenizer() else None
+        out = []
+        for s in searches:
+            found = [BeamHypothesis(decode(h.tokens, skip_special_tokens=True) if decode else "", h.tokens, h.sum_logprobs,
+                                    h.score(params.length_penalty), FinishReason.STOP if h.ended else FinishReason.LENGTH)
+                     for h in s.hypotheses(params)]
+            prompt = texts[s.index] if texts else decode(s.prompt, skip_special_tokens=True) if decode else None
+            out.append(BeamSearchOutput(s.index, prompt, s.prompt, found))
+        return out
 
     def _launch(self, plan: StepPlan) -> "_Flight":
         """Start one planned step.

@@ -25,3 +25,27 @@ class RequestOutput:
     ttft_s: float | None = None
     latency_s: float | None = None
     num_preemptions: int = 0
+
+
+@dataclass(frozen=True, slots=True)
+class BeamHypothesis:
+    """One continuation that a search over beams returns.
+
+    ``cumulative_logprob`` is the sum of the tokens' log probabilities, ``score`` that over the number of tokens to the
+    power of the length penalty; ``output_token_ids`` includes a final EOS if one ended it."""
+
+    output_text: str
+    output_token_ids: list[int]
+    cumulative_logprob: float
+    score: float
+    finish_reason: FinishReason
+
+
+@dataclass(frozen=True, slots=True)
+class BeamSearchOutput:
+    """The hypotheses of one prompt's search, best first."""
+
+    request_id: int
+    prompt: str | None
+    prompt_token_ids: list[int]
+    hypotheses: list[BeamHypothesis]

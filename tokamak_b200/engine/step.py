@@ -101,6 +101,7 @@ class StepBatch:
                             # that what kernels plan from it (grids, key splits) changes rarely
     scratch: dict = field(default_factory=dict)     # per-step values that parts share (e.g. plans)
     row_slot: torch.Tensor | None = None            # slot of the request of every wanted row
+    shared: "ops.SharedPrefix | None" = None        # positions that the requests of a step of single next tokens share
 
 
 @dataclass

@@ -92,6 +92,7 @@ class Attention:
     def weight_bytes(self) -> int:
         return tensor_bytes(self.w_qkv, self.w_o, self.q_norm_w, self.k_norm_w)
 
+    SHARED_PREFIX = True       # single next tokens may read keys that their requests share
     TAKES_OWED_NORM = True     # the q|k|v product pays an owed norm scale in its epilogue
     TAKES_THEN_NORM = True     # the output product can add itself to the residual stream
 
@@ -180,6 +181,8 @@ class CappedAttention:
     are one kernel (``csrc/qkv_pairs.cu``); scores, softmax and the weighted sum run in float32
     inside the attention kernels.
     """
+
+    SHARED_PREFIX = True
 
     def __init__(self, spec: CappedAttentionSpec, prefix: str, tensors: dict[str, torch.Tensor], rt: Runtime):
         if spec.num_heads % spec.num_kv_heads:
@@ -625,13 +628,20 @@ def paged_attention(q: torch.Tensor, out: torch.Tensor, cache_view, step, *, sca
     kernels and the tcgen05 prefill kernel.  ``dist_bias`` (float32 ``[Hq, L]``: the score of the key ``n``
     positions back gains ``dist_bias[h, min(n, L - 1)]``) is known to the same kernels.
 
-    Chooses the kernels.  A latent cache in bfloat16 goes to the tensor-core kernel that stacks the heads
+    Chooses the kernels.  Single next tokens whose requests share keys (``step.shared``) go to the shared-prefix kernels, which
+    know windows, caps and sinks.  A latent cache in bfloat16 goes to the tensor-core kernel that stacks the heads
     of a token (``csrc/attention_latent.cu``).  bfloat16 with a head_dim the tiled kernels take: single next
     tokens go to the split-K decode kernel, portions of prompts to the tcgen05 flash
     prefill kernel (or to the mma.sync one for page sizes it does not take).  float32,
     and every other shape, runs on the general kernel.
     """
     ops.flush_chains()     # q and the pages may come from a product that is still queued: launch it on this stream
+    if step.shared is not None:
+        if chunk is not None or slopes is not None or dist_bias is not None:
+            raise ops.KernelError("attention with chunks or distance biases does not know keys that requests share")
+        ops.attention_shared(q, out, cache_view.k, cache_view.v, step.shared, step.positions, step.req_slot, cache_view.table,
+                             step.err, scale=scale, window=window, softcap=softcap, sinks=sinks)
+        return
     n, hq, d = q.shape
     hkv, page = cache_view.k.shape[1], cache_view.k.shape[2]
     bf16 = q.dtype == torch.bfloat16

@@ -47,6 +47,9 @@ CUDA graph only if every part of the model says so; a model with one part that d
 ``weight_bytes()`` returns the bytes of the tensors that one call of the part reads in full
 (an embedding table, read by row, reports 0); measurements sum it over the schedule.
 
+``SHARED_PREFIX = True`` (an attention mixer) says that the mixer hands a step of single next tokens whose requests share
+keys (``step.shared``) to a kernel that knows them.  Search over beams runs on models whose mixers with pages all say so.
+
 ``prefill_heads`` (a mixer, or a block on its mixer's behalf) is a hint, not a contract: how many
 work items the part makes of one block of prompt tokens (an attention mixer: its query heads).
 The step function balances the work list of prompt portions (``step.prefill_tc``) for the smallest

@@ -1,3 +1,4 @@
+from .beam import BeamSearchParams
 from .params import SamplingParams
 
-__all__ = ["SamplingParams"]
+__all__ = ["BeamSearchParams", "SamplingParams"]
