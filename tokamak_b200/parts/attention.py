@@ -636,10 +636,11 @@ def paged_attention(q: torch.Tensor, out: torch.Tensor, cache_view, step, *, sca
     and every other shape, runs on the general kernel.
     """
     ops.flush_chains()     # q and the pages may come from a product that is still queued: launch it on this stream
-    if step.shared is not None:
+    shared = getattr(step, "shared", None)
+    if shared is not None:
         if chunk is not None or slopes is not None or dist_bias is not None:
             raise ops.KernelError("attention with chunks or distance biases does not know keys that requests share")
-        ops.attention_shared(q, out, cache_view.k, cache_view.v, step.shared, step.positions, step.req_slot, cache_view.table,
+        ops.attention_shared(q, out, cache_view.k, cache_view.v, shared, step.positions, step.req_slot, cache_view.table,
                              step.err, scale=scale, window=window, softcap=softcap, sinks=sinks)
         return
     n, hq, d = q.shape

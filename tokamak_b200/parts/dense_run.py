@@ -107,7 +107,8 @@ def run_layers(calls, resid: torch.Tensor, pending, step, next_norm):
     ms, fs, dtype = m.spec, f.spec, first.norm1.rt.dtype
     n, hidden, inter, d = step.n_tokens, ms.hidden_size, fs.intermediate_size, ms.head_dim
     hq, hkv = ms.num_heads, ms.num_kv_heads
-    if step.shared is not None or ops.CHAIN_POLICY == "on" or not resid.is_cuda or dtype not in ops.DTYPE_CODE or view.k.dtype != dtype:
+    if (getattr(step, "shared", None) is not None or ops.CHAIN_POLICY == "on" or not resid.is_cuda
+            or dtype not in ops.DTYPE_CODE or view.k.dtype != dtype):
         return pending, 0
     table, rotary_dim = m.position.rotary_table(step)
     few = dtype == torch.bfloat16 and n <= SWAPPED_GEMM_MAX_TOKENS
