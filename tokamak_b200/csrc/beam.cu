@@ -6,7 +6,8 @@
 // and the K largest keys of a group's W * V are wanted in order; equal keys of one beam by the larger logit, others by the
 // lowest w * V + v.  Keys of neighbouring ranks differ by less than a float's last place often enough to change what a
 // search does, so sums and keys are 64-bit: the exponentials are floats (an error of some 1e-7 each that falls away in the
-// sum, where the largest terms are exact or nearly so), added four at a time as floats and then as doubles.
+// sum, where the largest terms, those of the candidates, are put right in 64 bits), added four at a time as floats and then as
+// doubles.
 //
 // One pass over the logits.  Within a row the order of the keys is that of the logits, so the K best of a row's segment can
 // be kept without knowing the row's sum: a block streams its segment in tiles, holds a threshold with at least K elements
@@ -21,11 +22,12 @@
 
 namespace tk {
 
-constexpr int kSelThreads = 512;
-constexpr int kSelVecs = 2;                                    // 16-byte loads of a thread in one tile
-constexpr int kSelTile = kSelThreads * 4 * kSelVecs;           // logits of a tile
-constexpr int kSelBuffer = 2 * kSelTile;                       // elements set aside: a whole tile always fits behind what is kept
-constexpr int kSelRanked = kSelThreads;                        // so many are ranked by comparing each with each
+constexpr int kSelThreads = 256;
+constexpr int kSelEach = 16;                                   // logits of a thread in one tile
+constexpr int kSelTile = kSelThreads * kSelEach;               // logits of a tile
+constexpr int kSelKept = 512;                                  // elements set aside that are left when they are thinned out
+constexpr int kSelBuffer = 2048;                               // elements set aside
+constexpr int kJoinThreads = 512;                              // and so many are ranked by comparing each with each
 constexpr int kSelMaxK = 256;
 constexpr int kSelMaxBeams = 64;
 constexpr int kSelMaxEntries = 16384;                          // beams * segments * K that a joining block takes
@@ -63,21 +65,19 @@ __device__ __forceinline__ bool dead_score(float s) { return !(s > -INFINITY); }
 
 // The largest threshold, bit by bit from the top, with at least k of the block's values at or above it; it stops early at one
 // with at most `most`.  count(t) gives this thread's values at or above t.
-template <typename U, typename Count>
+template <int kThreads, typename U, typename Count>
 __device__ __forceinline__ U block_threshold(int k, int most, Count count) {
+  __shared__ int s_warp[2][kThreads / 32];
   U t = 0;
   for (int bit = 8 * (int)sizeof(U) - 1; bit >= 0; --bit) {
     const U trial = t | ((U)1 << bit);
-    // a thread's count may exceed one: the warps' sums are added up by the barrier's own reduction, bit by bit
-    const int mine = count(trial);
-    __shared__ int s_warp[2][kSelThreads / 32];
-    const int sum = __reduce_add_sync(0xffffffffu, mine);
+    const int sum = __reduce_add_sync(0xffffffffu, count(trial));
     int* w = s_warp[bit & 1];
     if ((threadIdx.x & 31) == 0) w[threadIdx.x >> 5] = sum;
     __syncthreads();
     int total = 0;
 #pragma unroll
-    for (int i = 0; i < kSelThreads / 32; ++i) total += w[i];
+    for (int i = 0; i < kThreads / 32; ++i) total += w[i];
     if (total >= k) {
       t = trial;
       if (total <= most) break;
@@ -87,16 +87,33 @@ __device__ __forceinline__ U block_threshold(int k, int most, Count count) {
   return t;
 }
 
-// Keeps the k largest (and a few behind them, up to kSelRanked) of the n distinct elements set aside; returns how many.
-__device__ __forceinline__ int thin_out(unsigned long long* buf, int* s_count, int n, int k) {
+// The same with one value a thread, which the barrier itself counts.
+template <typename U>
+__device__ __forceinline__ U block_threshold_of(int k, int most, bool any, U value) {
+  U t = 0;
+  for (int bit = 8 * (int)sizeof(U) - 1; bit >= 0; --bit) {
+    const U trial = t | ((U)1 << bit);
+    const int total = __syncthreads_count(any && value >= trial);
+    if (total >= k) {
+      t = trial;
+      if (total <= most) break;
+    }
+  }
+  return t;
+}
+
+// Of the n elements set aside those of tokens before `limit` are kept, and of these, where they are more than kSelKept, the k
+// largest (and a few behind them, up to kSelKept).  Returns how many.  (Elements are distinct.)
+__device__ __noinline__ int thin_out(unsigned long long* buf, int* s_count, int n, int k, unsigned int limit) {
   constexpr int PER = kSelBuffer / kSelThreads;
   unsigned long long mine[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int at = i * kSelThreads + threadIdx.x;
     mine[i] = at < n ? buf[at] : 0ull;
+    if (0xffffffffu - (unsigned int)mine[i] >= limit) mine[i] = 0ull;
   }
-  const unsigned long long t = block_threshold<unsigned long long>(k, kSelRanked, [&](unsigned long long trial) {
+  const unsigned long long t = block_threshold<kSelThreads, unsigned long long>(k, kSelKept, [&](unsigned long long trial) {
     int c = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) c += mine[i] >= trial ? 1 : 0;
@@ -112,19 +129,58 @@ __device__ __forceinline__ int thin_out(unsigned long long* buf, int* s_count, i
   return *s_count;
 }
 
-__global__ void __launch_bounds__(kSelThreads)
+// The smallest logit of the n elements set aside (at most kSelKept), as a float.
+__device__ __forceinline__ float lowest_of(const unsigned long long* buf, int n) {
+  __shared__ unsigned int s_low[kSelThreads / 32];
+  unsigned int low = 0xffffffffu;
+  for (int i = threadIdx.x; i < n; i += kSelThreads) low = min(low, (unsigned int)(buf[i] >> 32));
+  low = __reduce_min_sync(0xffffffffu, low);
+  if ((threadIdx.x & 31) == 0) s_low[threadIdx.x >> 5] = low;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSelThreads / 32; ++i) low = min(low, s_low[i]);
+  __syncthreads();
+  return from_ordered_f32(low);
+}
+
+// s_rank[j] (zero before) becomes the number of the n elements that come before element j: as many threads as there are work on
+// each of up to a block's threads, or a thread on several.
+template <int kThreads, typename Before>
+__device__ __forceinline__ void rank_by_slices(int n, int* s_rank, Before before) {
+  const int slices = max(1, kThreads / max(1, n));
+  const int slice = (int)threadIdx.x / max(1, n);
+  if (slice < slices) {
+    for (int j = slice == 0 ? (int)threadIdx.x : (int)threadIdx.x % n; j < n; j += kThreads) {
+      int c = 0;
+      for (int i = slice; i < n; i += slices) c += before(i, j) ? 1 : 0;
+      if (slices > 1) atomicAdd(&s_rank[j], c);
+      else s_rank[j] = c;
+    }
+  }
+  __syncthreads();
+}
+
+// Exponentials as the sums take them: a subtraction that is exact for the terms that matter, a product, and the fast power of two.
+__device__ __forceinline__ float2 terms_f32(float x, float y, float ref) {
+  float2 d = mul2(add2(make_float2(x, y), make_float2(-ref, -ref)), make_float2(1.4426950408889634f, 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(d.x));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(d.y));
+  return d;
+}
+
+__global__ void __launch_bounds__(kSelThreads, 4)
 beam_segments_kernel(SelectParams p) {
   pdl_trigger();
-  extern __shared__ unsigned long long s_buf[];                // [kSelBuffer]
-  __shared__ int s_count;
+  __shared__ unsigned long long s_buf[kSelBuffer];
+  __shared__ int s_count, s_rank[kSelKept];
   __shared__ float s_max[kSelThreads / 32];
-  __shared__ double s_sum[kSelThreads / 32];
+  __shared__ double s_sum[kSelThreads / 32], s_late[kSelMaxK];
   const int seg = blockIdx.x;
   const long long row = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const size_t at_part = (size_t)row * p.segments + seg;
   unsigned long long* out = p.seg_key + at_part * p.k;
-  const int begin = seg * p.seg_len, end = min(p.vocab, begin + p.seg_len);
+  const int begin = min(p.vocab, seg * p.seg_len), end = min(p.vocab, begin + p.seg_len);
   pdl_wait();
   if (dead_score(p.scores[row])) {
     // the first tokens stand for a beam that cannot go on
@@ -135,113 +191,116 @@ beam_segments_kernel(SelectParams p) {
     return;
   }
   const float* x = p.logits + row * p.ld;
-  // 16-byte loads on their boundaries, wherever the row begins; what lies outside the segment is not read
-  const int shift = (int)(((uintptr_t)x >> 2) & 3);
-  const int v_begin = (begin + shift) / 4, v_end = (end + shift + 3) / 4;
-  auto load = [&](int v, float (&e)[4]) {
-    const int i0 = 4 * v - shift;
-    if (i0 >= begin && i0 + 4 <= end) {
-      const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i0));
-      e[0] = f.x; e[1] = f.y; e[2] = f.z; e[3] = f.w;
+  // A thread takes every kSelThreads-th logit of a tile, wherever the row begins: two rows with the same logits have the same
+  // sum to the last bit then, whatever their addresses, and their continuations are ties.
+  auto load_tile = [&](int t0, float (&e)[kSelEach]) {
+    const float* src = x + t0 + threadIdx.x;
+    if (t0 + kSelTile <= end) {
+#pragma unroll
+      for (int j = 0; j < kSelEach; ++j) e[j] = __ldcs(src + j * kSelThreads);
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) e[j] = (i0 + j >= begin && i0 + j < end) ? x[i0 + j] : -INFINITY;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) e[j] = fmaxf(e[j], -INFINITY);          // a NaN becomes -inf
-  };
-  float e[kSelVecs][4];
-  auto load_tile = [&](int v0) {
-#pragma unroll
-    for (int u = 0; u < kSelVecs; ++u) {
-      const int v = v0 + u * kSelThreads + (int)threadIdx.x;
-      if (v < v_end) load(v, e[u]);
-      else e[u][0] = e[u][1] = e[u][2] = e[u][3] = -INFINITY;
+      for (int j = 0; j < kSelEach; ++j) e[j] = t0 + j * kSelThreads + (int)threadIdx.x < end ? src[j * kSelThreads] : -INFINITY;
     }
   };
-  auto tile_max = [&]() {
-    float m = -INFINITY;
+  auto clean = [&](float (&e)[kSelEach]) {                        // a NaN becomes -inf
 #pragma unroll
-    for (int u = 0; u < kSelVecs; ++u) m = fmaxf(m, fmaxf(fmaxf(e[u][0], e[u][1]), fmaxf(e[u][2], e[u][3])));
+    for (int j = 0; j < kSelEach; ++j) e[j] = fmaxf(e[j], -INFINITY);
+  };
+  auto tile_max = [&](const float (&e)[kSelEach]) {
+    float m = fmaxf(e[0], e[1]);
+#pragma unroll
+    for (int j = 2; j < kSelEach; j += 2) m = fmaxf(m, fmaxf(e[j], e[j + 1]));
     return m;
   };
-  auto set_aside = [&](int v0, unsigned int least, bool strict) {
-#pragma unroll
-    for (int u = 0; u < kSelVecs; ++u) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = 4 * (v0 + u * kSelThreads + (int)threadIdx.x) - shift + j;
-        const unsigned int o = ordered_f32(e[u][j]);
-        if (i >= begin && i < end && (strict ? o > least : o >= least)) {
-          s_buf[atomicAdd(&s_count, 1)] = ((unsigned long long)o << 32) | (0xffffffffu - (unsigned)i);
-        }
-      }
-    }
+  auto set_aside = [&](int i, float v) {
+    const int at = atomicAdd(&s_count, 1);
+    if (at < kSelBuffer) s_buf[at] = ((unsigned long long)ordered_f32(v) << 32) | (0xffffffffu - (unsigned)i);
   };
 
   // ---- the first tile: a reference for the sums, and a threshold -----------------------------------------------
   if (threadIdx.x == 0) s_count = 0;
-  load_tile(v_begin);
-  float top = tile_max();
+  float cur[kSelEach], nxt[kSelEach];
+  load_tile(begin, cur);
+  if (begin + kSelTile < end) load_tile(begin + kSelTile, nxt);
+  clean(cur);
+  const float top = tile_max(cur);
   {
     const float w = warp_max(top);
     if (lane == 0) s_max[warp] = w;
   }
-  const unsigned int o_top = ordered_f32(top);
-  const bool any = 4 * (v_begin + (int)threadIdx.x) - shift < end;
-  unsigned int least = block_threshold<unsigned int>(p.k, p.k + 32, [&](unsigned int t) { return any && o_top >= t ? 1 : 0; });
+  const unsigned int o_least = block_threshold_of<unsigned int>(p.k, p.k, begin + (int)threadIdx.x < end, ordered_f32(top));
   float ref = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kSelThreads / 32; ++i) ref = fmaxf(ref, s_max[i]);
-  set_aside(v_begin, least, false);
+  // elements at or above this are set aside in the first tile, those above it in later ones: what is equal and comes later
+  // loses.  (At or below -inf's place: fewer than K threads have an element that is more.)
+  float least = o_least <= ordered_f32(-INFINITY) ? -INFINITY : from_ordered_f32(o_least);
   double sum = 0.0;
-  float least_f = from_ordered_f32(least);        // 0 (fewer than K elements in all) is below every float's place: a NaN
-  if (least == 0u) least_f = -INFINITY;
 
-  // The sum of this tile's exponentials.  The reference is the first tile's maximum; it is raised (and what has been
+  // More elements than the buffer holds: those of the tile are set aside again, a row of a block's threads at a time, with the
+  // threshold raised in between.  (Logits in rising order, or many equal ones.)
+  auto crowded = [&](int t0, const float (&e)[kSelEach], bool first) {
+    __syncthreads();
+    int n = thin_out(s_buf, &s_count, min(s_count, kSelBuffer), p.k, (unsigned int)t0);
+    bool reached = first;                         // whether an element equal to the threshold still counts
+    if (n >= p.k) { least = lowest_of(s_buf, n); reached = false; }
+#pragma unroll
+    for (int j = 0; j < kSelEach; ++j) {
+      const int i = t0 + j * kSelThreads + (int)threadIdx.x;
+      if (i < end && (reached ? e[j] >= least : e[j] > least)) set_aside(i, e[j]);
+      __syncthreads();
+      n = s_count;
+      __syncthreads();
+      if (n > kSelBuffer - kSelThreads) {
+        n = thin_out(s_buf, &s_count, n, p.k, 0xffffffffu);
+        least = lowest_of(s_buf, n);
+        reached = false;
+      }
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < kSelEach; ++j) {
+    if (cur[j] >= least && begin + j * kSelThreads + (int)threadIdx.x < end) set_aside(begin + j * kSelThreads + (int)threadIdx.x, cur[j]);
+  }
+  if (__syncthreads_or(s_count > kSelBuffer)) crowded(begin, cur, true);
+
+  // The sum of a tile's exponentials.  The reference is the first tile's maximum; it is raised (and what has been
   // summed so far scaled down) only where an exponent would leave the range that the sums hold.
-  auto add_tile = [&]() {
-    const float m = tile_max();
+  auto add_tile = [&](const float (&e)[kSelEach], float m) {
     if (!(m - ref <= kSelRaise)) {                // also with a reference of -inf or +inf
       if (m == -INFINITY) return;
       if (m == INFINITY || ref == INFINITY) {     // from the first +inf on these are counted, and nothing else
         if (ref != INFINITY) { sum = 0.0; ref = INFINITY; }
 #pragma unroll
-        for (int u = 0; u < kSelVecs; ++u) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sum += e[u][j] == INFINITY ? 1.0 : 0.0;
-        }
+        for (int j = 0; j < kSelEach; ++j) sum += e[j] == INFINITY ? 1.0 : 0.0;
         return;
       }
       sum = ref == -INFINITY ? 0.0 : sum * exp((double)ref - (double)m);
       ref = m;
     }
 #pragma unroll
-    for (int u = 0; u < kSelVecs; ++u) {
-      const float a = expf(e[u][0] - ref) + expf(e[u][1] - ref), b = expf(e[u][2] - ref) + expf(e[u][3] - ref);
-      sum += (double)(a + b);
+    for (int j = 0; j < kSelEach; j += 4) {
+      const float2 a = terms_f32(e[j], e[j + 1], ref), b = terms_f32(e[j + 2], e[j + 3], ref);
+      const float2 c = add2(a, b);
+      sum += (double)(c.x + c.y);
     }
   };
-  add_tile();
-  for (int v0 = v_begin + kSelThreads * kSelVecs; v0 < v_end; v0 += kSelThreads * kSelVecs) {
-    load_tile(v0);
-    if (tile_max() > least_f) set_aside(v0, least, true);
-    add_tile();
-    if (__syncthreads_or(s_count > kSelBuffer - kSelTile)) {
-      // many elements in rising order: keep the best and raise the threshold
-      int n = s_count;
-      __syncthreads();
-      n = thin_out(s_buf, &s_count, n, p.k);
-      unsigned int lowest = threadIdx.x < n ? (unsigned int)(s_buf[threadIdx.x] >> 32) : 0xffffffffu;
-      lowest = __reduce_min_sync(0xffffffffu, lowest);
-      if (lane == 0) s_max[warp] = __uint_as_float(lowest);
-      __syncthreads();
-      least = 0xffffffffu;
+  add_tile(cur, top);
+  for (int t0 = begin + kSelTile; t0 < end; t0 += kSelTile) {
 #pragma unroll
-      for (int i = 0; i < kSelThreads / 32; ++i) least = min(least, __float_as_uint(s_max[i]));
-      least_f = from_ordered_f32(least);
-      __syncthreads();
+    for (int j = 0; j < kSelEach; ++j) cur[j] = nxt[j];
+    if (t0 + kSelTile < end) load_tile(t0 + kSelTile, nxt);
+    clean(cur);
+    const float m = tile_max(cur);
+    if (m > least) {                              // -inf behind the segment's end is never more
+#pragma unroll
+      for (int j = 0; j < kSelEach; ++j) {
+        if (cur[j] > least) set_aside(t0 + j * kSelThreads + (int)threadIdx.x, cur[j]);
+      }
     }
+    add_tile(cur, m);
+    if (__syncthreads_or(s_count > kSelBuffer)) crowded(t0, cur, false);
   }
   __syncthreads();
 
@@ -252,14 +311,34 @@ beam_segments_kernel(SelectParams p) {
   }
   int n = s_count;
   __syncthreads();
+  if (n > kSelKept) n = thin_out(s_buf, &s_count, n, p.k, 0xffffffffu);
   float ref_all = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kSelThreads / 32; ++i) ref_all = fmaxf(ref_all, s_max[i]);
-  if (ref != ref_all) sum = (ref == -INFINITY || ref_all == INFINITY) ? 0.0 : sum * exp((double)ref - (double)ref_all);
+  const bool same = ref == ref_all;
+  if (!same) sum = (ref == -INFINITY || ref_all == INFINITY) ? 0.0 : sum * exp((double)ref - (double)ref_all);
+  // Where no thread raised its reference, the K best, which the sum is mostly made of, are summed in 64 bits after all: what their
+  // fast exponentials were off by is added.
+  const bool one_ref = __syncthreads_and(same) && ref_all > -INFINITY && ref_all < INFINITY;
+  if ((int)threadIdx.x < p.k) s_late[threadIdx.x] = 0.0;
+  for (int i = threadIdx.x; i < kSelKept; i += kSelThreads) s_rank[i] = 0;
+  __syncthreads();
+  rank_by_slices<kSelThreads>(n, s_rank, [&](int i, int j) { return s_buf[i] > s_buf[j]; });
+  for (int i = threadIdx.x; i < n; i += kSelThreads) {
+    const unsigned long long mine = s_buf[i];
+    const int rank = s_rank[i];
+    if (rank < p.k) {
+      out[rank] = mine;
+      const float v = from_ordered_f32((unsigned int)(mine >> 32));
+      if (one_ref && v > -INFINITY) s_late[rank] = exp((double)v - (double)ref_all) - (double)terms_f32(v, v, ref_all).x;
+    }
+  }
+  for (int i = n + (int)threadIdx.x; i < p.k; i += kSelThreads) out[i] = 0ull;
+  __syncthreads();
+  if ((int)threadIdx.x < p.k) sum += s_late[threadIdx.x];        // by rank: the order of the additions is always the same
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s_sum[warp] = sum;
-  if (n > kSelRanked) n = thin_out(s_buf, &s_count, n, p.k);
   __syncthreads();
   if (threadIdx.x == 0) {
     double total = 0.0;
@@ -267,42 +346,38 @@ beam_segments_kernel(SelectParams p) {
     p.seg_sum[2 * at_part] = (double)ref_all;
     p.seg_sum[2 * at_part + 1] = total;
   }
-  if ((int)threadIdx.x < n) {
-    const unsigned long long mine = s_buf[threadIdx.x];
-    int rank = 0;
-    for (int i = 0; i < n; ++i) rank += s_buf[i] > mine ? 1 : 0;
-    if (rank < p.k) out[rank] = mine;
-  }
-  for (int i = n + (int)threadIdx.x; i < p.k; i += kSelThreads) out[i] = 0ull;
 }
 
-// One block per group: the sums of its rows, the keys of the elements set aside, the K best of them in order.
-__global__ void __launch_bounds__(kSelThreads)
+// One block per group: the sums of its rows, the keys of the elements set aside, the K best of them in order.  A segment's elements
+// come best first, so where there are more segments than K only those whose first is among the K best firsts matter.
+__global__ void __launch_bounds__(kJoinThreads)
 beam_join_kernel(SelectParams p) {
   pdl_trigger();
   extern __shared__ unsigned long long s_key[];                // [beams * segments * K] keys in their order
   __shared__ double s_ref[kSelMaxBeams], s_log[kSelMaxBeams];
-  __shared__ unsigned long long s_best[kSelRanked];
-  __shared__ unsigned long long s_second[kSelRanked];
-  __shared__ int s_count;
+  __shared__ unsigned long long s_best[kJoinThreads];
+  __shared__ unsigned long long s_second[kJoinThreads];
+  __shared__ int s_count, s_rank[kJoinThreads];
   const int group = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const size_t row0 = (size_t)group * p.beams;
   const int per_row = p.segments * p.k;
-  const int n = p.beams * per_row;
+  const int n = p.beams * per_row, lists = p.beams * p.segments;
   if (threadIdx.x == 0) s_count = 0;
+  s_rank[threadIdx.x] = 0;
   pdl_wait();
-  for (int b = warp; b < p.beams; b += kSelThreads / 32) {
-    const double* seg = p.seg_sum + (row0 + b) * p.segments * 2;
-    double ref = -INFINITY;
-    for (int s = lane; s < p.segments; s += 32) ref = fmax(ref, __ldcg(seg + 2 * s));
+  for (int b = warp; b < p.beams; b += kJoinThreads / 32) {
+    const double2* seg = reinterpret_cast<const double2*>(p.seg_sum) + (row0 + b) * p.segments;
+    const double2 first = lane < p.segments ? __ldcg(seg + lane) : make_double2(-INFINITY, 0.0);
+    double ref = first.x;
+    for (int s = lane + 32; s < p.segments; s += 32) ref = fmax(ref, __ldcg(seg + s).x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ref = fmax(ref, __shfl_xor_sync(0xffffffffu, ref, o));
     double sum = 0.0;
     for (int s = lane; s < p.segments; s += 32) {
-      const double m = __ldcg(seg + 2 * s), part = __ldcg(seg + 2 * s + 1);
-      if (m == ref) sum += part;
-      else if (m != -INFINITY && ref != INFINITY) sum += part * exp(m - ref);
+      const double2 part = s == lane ? first : __ldcg(seg + s);
+      if (part.x == ref) sum += part.y;
+      else if (part.x != -INFINITY && ref != INFINITY) sum += part.y * exp(part.x - ref);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -318,9 +393,34 @@ beam_join_kernel(SelectParams p) {
     return ordered_f64(key);
   };
   const unsigned long long* elems = p.seg_key + row0 * per_row;
-  for (int i = threadIdx.x; i < n; i += kSelThreads) {
+  auto any_key = [&](int i) {
     const unsigned long long elem = __ldcg(elems + i);
-    s_key[i] = elem == 0ull ? 0ull : key_of(i / per_row, elem);
+    return elem == 0ull ? 0ull : key_of(i / per_row, elem);
+  };
+  // Keys as floats, rounded down, are in the keys' order but for what they round away, and half the bits to look at.
+  auto as_float = [&](unsigned long long key) { return key == 0ull ? 0u : ordered_f32(__double2float_rd(from_ordered_f64(key))); };
+  auto from_float = [&](unsigned int t32) { return t32 <= ordered_f32(-INFINITY) ? 1ull : ordered_f64((double)from_ordered_f32(t32)); };
+  unsigned long long t = 1ull;                                   // everything there is
+  if (lists > p.k) {
+    for (int i = threadIdx.x; i < lists; i += kJoinThreads) s_key[i * p.k] = any_key(i * p.k);
+    __syncthreads();
+    if (lists <= kJoinThreads) {
+      const unsigned long long key = (int)threadIdx.x < lists ? s_key[threadIdx.x * p.k] : 0ull;
+      t = from_float(block_threshold_of<unsigned int>(p.k, p.k, key != 0ull, as_float(key)));
+    } else {
+      t = from_float(block_threshold<kJoinThreads, unsigned int>(p.k, p.k + p.k / 4, [&](unsigned int trial) {
+        int c = 0;
+        for (int i = threadIdx.x; i < lists; i += kJoinThreads) c += as_float(s_key[i * p.k]) >= trial ? 1 : 0;
+        return c;
+      }));
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kJoinThreads) {
+      const int list = i / p.k, first = list * p.k;
+      if (i != first) s_key[i] = s_key[first] >= t ? any_key(i) : 0ull;
+    }
+  } else {
+    for (int i = threadIdx.x; i < n; i += kJoinThreads) s_key[i] = any_key(i);
   }
   __syncthreads();
   // what comes after the key: the logit where it decides, then the place
@@ -330,50 +430,81 @@ beam_join_kernel(SelectParams p) {
     const unsigned int logit = s_key[i] == ordered_f64(-INFINITY) ? 0u : (unsigned int)(elem >> 32);
     return ((unsigned long long)logit << 32) | (0xffffffffu - place);
   };
-  unsigned long long t = 1ull;                                   // everything there is
-  if (n > kSelRanked) {
-    t = block_threshold<unsigned long long>(p.k, kSelRanked, [&](unsigned long long trial) {
-      int c = 0;
-      for (int i = threadIdx.x; i < n; i += kSelThreads) c += s_key[i] >= trial ? 1 : 0;
-      return c;
-    });
-    if (t == 0ull) t = 1ull;
-  }
-  // Where more than can be ranked share the K-th key (beams that all are dead, rows of equal logits), the same search goes on
-  // over what comes after the key.
-  int mine = 0, above = 0;
-  for (int i = threadIdx.x; i < n; i += kSelThreads) { mine += s_key[i] >= t ? 1 : 0; above += s_key[i] > t ? 1 : 0; }
-  unsigned long long t2 = 0ull;
-  {
-    __shared__ int s_sums[2][kSelThreads / 32];
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    above = __reduce_add_sync(0xffffffffu, above);
-    if (lane == 0) { s_sums[0][warp] = mine; s_sums[1][warp] = above; }
+  auto gather = [&](unsigned long long t, unsigned long long t2) {
     __syncthreads();
-    mine = above = 0;
-#pragma unroll
-    for (int i = 0; i < kSelThreads / 32; ++i) { mine += s_sums[0][i]; above += s_sums[1][i]; }
-  }
-  if (mine > kSelRanked) {
-    t2 = block_threshold<unsigned long long>(p.k - above, kSelRanked - above, [&](unsigned long long trial) {
-      int c = 0;
-      for (int i = threadIdx.x; i < n; i += kSelThreads) c += (s_key[i] == t && second_of(i) >= trial) ? 1 : 0;
-      return c;
-    });
-  }
-  for (int i = threadIdx.x; i < n; i += kSelThreads) {
-    if (s_key[i] > t || (s_key[i] == t && (t2 == 0ull || second_of(i) >= t2))) {
-      const int at = atomicAdd(&s_count, 1);
-      s_best[at] = s_key[i];
-      s_second[at] = second_of(i);
+    if (threadIdx.x == 0) s_count = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kJoinThreads) {
+      const unsigned long long key = s_key[i];
+      if (key < t) continue;
+      const unsigned long long second = second_of(i);
+      if (key > t || second >= t2) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kJoinThreads) { s_best[at] = key; s_second[at] = second; }
+      }
     }
+    __syncthreads();
+    return s_count;
+  };
+  int m = gather(t, 0ull);
+  if (m > kJoinThreads) {
+    // more than can be ranked: a threshold over all of them
+    t = max(t, from_float(block_threshold<kJoinThreads, unsigned int>(p.k, kJoinThreads, [&](unsigned int trial) {
+      int c = 0;
+      for (int i = threadIdx.x; i < n; i += kJoinThreads) c += as_float(s_key[i]) >= trial ? 1 : 0;
+      return c;
+    })));
+    m = gather(t, 0ull);
   }
-  __syncthreads();
-  const int m = s_count;
+  if (m > kJoinThreads) {
+    // Where more than can be ranked share the K-th key (beams that all are dead, rows of equal logits), the same search goes on
+    // over all bits of the keys, and then over what comes after the key.
+    auto at_least = [&](unsigned long long trial) {
+      int c = 0;
+      for (int i = threadIdx.x; i < n; i += kJoinThreads) c += s_key[i] >= trial ? 1 : 0;
+      return c;
+    };
+    t = max(1ull, block_threshold<kJoinThreads, unsigned long long>(p.k, kJoinThreads, at_least));
+    unsigned long long t2 = 0ull;
+    __shared__ int s_above;
+    if (threadIdx.x == 0) s_above = 0;
+    __syncthreads();
+    const int above_here = at_least(t + 1ull);
+    if (above_here > 0) atomicAdd(&s_above, above_here);
+    __syncthreads();
+    const int above = s_above;
+    if (above < p.k) {
+      t2 = block_threshold<kJoinThreads, unsigned long long>(p.k - above, kJoinThreads - above, [&](unsigned long long trial) {
+        int c = 0;
+        for (int i = threadIdx.x; i < n; i += kJoinThreads) c += (s_key[i] == t && second_of(i) >= trial) ? 1 : 0;
+        return c;
+      });
+    }
+    m = gather(t, t2);
+  }
+  if (m > 64 && m > 2 * p.k) {
+    // ranking compares each with each: a threshold over them first
+    const bool there = (int)threadIdx.x < m;
+    const unsigned long long key = there ? s_best[threadIdx.x] : 0ull, second = there ? s_second[threadIdx.x] : 0ull;
+    const unsigned long long least = from_float(block_threshold_of<unsigned int>(p.k, p.k + p.k / 4, there, as_float(key)));
+    __syncthreads();
+    if (threadIdx.x == 0) s_count = 0;
+    __syncthreads();
+    if (there && key >= least) {
+      const int at = atomicAdd(&s_count, 1);
+      s_best[at] = key;
+      s_second[at] = second;
+    }
+    __syncthreads();
+    m = s_count;
+  }
+  rank_by_slices<kJoinThreads>(m, s_rank, [&](int i, int j) {
+    const unsigned long long a = s_best[i], b = s_best[j];
+    return a > b || (a == b && s_second[i] > s_second[j]);
+  });
   if ((int)threadIdx.x < m) {
     const unsigned long long a = s_best[threadIdx.x], b = s_second[threadIdx.x];
-    int rank = 0;
-    for (int i = 0; i < m; ++i) rank += (s_best[i] > a || (s_best[i] == a && s_second[i] > b)) ? 1 : 0;
+    const int rank = s_rank[threadIdx.x];
     if (rank < p.k) {
       const size_t at = (size_t)group * p.k + rank;
       const unsigned int place = 0xffffffffu - (unsigned int)b;
@@ -577,7 +708,6 @@ TK_API int tk_beam_select(const float* logits, long long ld, const float* scores
   p.out_scores = out_scores; p.out_parents = out_parents; p.out_tokens = out_tokens;
   p.beams = beams; p.vocab = vocab; p.k = k; p.segments = segments;
   p.seg_len = (vocab + segments - 1) / segments;
-  constexpr int seg_smem = tk::kSelBuffer * 8;
   const int join_smem = beams * segments * k * 8;
   static bool configured[64] = {false};
   int dev = 0;
@@ -585,15 +715,13 @@ TK_API int tk_beam_select(const float* logits, long long ld, const float* scores
   if (e != cudaSuccess) return (int)e;
   if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidValue;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(tk::beam_segments_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, seg_smem);
-    if (e != cudaSuccess) return (int)e;
     e = cudaFuncSetAttribute(tk::beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tk::kSelMaxEntries * 8);
     if (e != cudaSuccess) return (int)e;
     configured[dev] = true;
   }
-  e = tk::launch(tk::beam_segments_kernel, dim3(segments, groups * beams), dim3(tk::kSelThreads), seg_smem, stream, p);
+  e = tk::launch(tk::beam_segments_kernel, dim3(segments, groups * beams), dim3(tk::kSelThreads), 0, stream, p);
   if (e != cudaSuccess) return (int)e;
-  return (int)tk::launch(tk::beam_join_kernel, dim3(groups), dim3(tk::kSelThreads), join_smem, stream, p);
+  return (int)tk::launch(tk::beam_join_kernel, dim3(groups), dim3(tk::kJoinThreads), join_smem, stream, p);
 }
 
 TK_API int tk_beam_advance(const float* cand_scores, const int* cand_parents, const int* cand_tokens, const int* stop_tokens,

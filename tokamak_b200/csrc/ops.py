@@ -237,11 +237,14 @@ _BEAM_TILE = 4096                 # logits that a block has in flight at a time
 BEAM_SEAT_LIMIT = 64              # seats of a group that reorder_slots moves between
 
 
-def beam_segments(device: torch.device, rows: int, beams: int, vocab: int, candidates: int) -> int:
-    """Segments that a row of logits is cut into: as many as fill the SMs with two blocks each, none shorter than a block's
-    tile, and no more than the joining kernel holds the candidates of."""
-    fill = 2 * sm_count(device) // max(1, rows)
-    return max(1, min(fill, -(-vocab // _BEAM_TILE), _BEAM_MAX_ENTRIES // (beams * candidates)))
+@lru_cache(maxsize=None)
+def beam_segments(sms: int, rows: int, beams: int, vocab: int, candidates: int) -> int:
+    """Segments that a row of logits is cut into.  Four blocks run on an SM at a time; a block costs its tiles and, for the first
+    threshold and the ranks, about as much as 6,000 logits more.  Taken is the number for which the rounds of blocks cost least, none
+    shorter than a block's tile, and no more than the joining kernel holds the candidates of."""
+    most = max(1, min(-(-vocab // _BEAM_TILE), _BEAM_MAX_ENTRIES // (beams * candidates)))
+    cost = lambda s: -(-rows * s // (4 * sms)) * (-(-vocab // s // _BEAM_TILE) * _BEAM_TILE + 6000)
+    return min(range(1, most + 1), key=cost)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int, *, out: tuple | None = None
@@ -284,7 +287,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int, *, 
     _want_here(logits=logits, scores=scores, out=out[0], parents=out[1], tokens=out[2])
     if groups == 0:
         return out
-    segments = beam_segments(logits.device, rows, beams, vocab, candidates)
+    segments = beam_segments(sm_count(logits.device), rows, beams, vocab, candidates)
     scratch = torch.empty(rows * segments * (2 + candidates), dtype=torch.int64, device=logits.device)
     _check(_lib().tk_beam_select(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, scores.data_ptr(),
                                  scratch.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), groups, beams,
