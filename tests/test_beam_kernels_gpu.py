@@ -341,7 +341,7 @@ class Shared:
     request may see filled with NaN."""
 
     def __init__(self, members, prefixes, own, *, hq=4, hkv=2, d=64, dv=None, page=16, dtype=torch.bfloat16, history=False, seed=0,
-                 window=None, softcap=None, sinks=False, lost_rows=0):
+                 window=None, softcap=None, sinks=False, common=0):
         rng = np.random.default_rng(seed)
         gen = torch.Generator().manual_seed(seed)
         self.hq, self.hkv, self.d, self.dv, self.page, self.dtype = hq, hkv, d, dv or d, page, dtype
@@ -382,6 +382,9 @@ class Shared:
             for r, g in enumerate(self.group_of):
                 start = int(np.cumsum([0] + list(members))[g])
                 for t in range(int(own[r]) - 1):
+                    if t < common:                       # the same writer for all members
+                        self.history[self.slots[r], t] = (7 * t + 3) % members[g]
+                        continue
                     able = [m for m in range(members[g]) if own[start + m] > t]
                     self.history[self.slots[r], t] = able[rng.integers(len(able))]
         self.k, self.v = k.to(dtype), v.to(dtype)
@@ -516,6 +519,33 @@ def test_shared_attention_long(dtype):
 def test_shared_attention_of_many_query_heads(members, dtype, d):
     """More (query head, member) pairs over a key head than a tile of rows, or two, hold."""
     c = Shared(members, [150, 70, 200][:len(members)], 21, hq=16, hkv=1, d=d, dtype=dtype, history=True, seed=14).device()
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("dtype,d,hq", [(torch.float32, 64, 4), (torch.bfloat16, 64, 4), (torch.bfloat16, 128, 4), (torch.bfloat16, 128, 32)])
+@pytest.mark.parametrize("members,prefixes,own,common,window", [
+    ([4], [100], 60, 59, None), ([4], [100], 60, 58, None), ([8, 3], [64, 130], 200, 150, None), ([5], [0], 90, 80, None), ([2], [1], 66, 64, None),
+    ([6], [200], 300, 290, 64), ([6], [200], 300, 290, 310), ([6], [200], 150, 140, 152), ([20], [300], 129, 127, None), ([4, 4], [33, 70], 2, 1, None),
+    ([3], [150], [140, 90, 120], 89, None)])
+def test_shared_attention_of_beams_with_a_common_past(members, prefixes, own, common, window, dtype, d, hq):
+    c = Shared(members, prefixes, own, hq=hq, hkv=2, d=d, dtype=dtype, history=True, common=common, window=window, seed=15).device()
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("d,hq,members,own", [(128, 16, [12], 400), (64, 16, [16, 2], 200), (128, 16, [40], [70 * (i % 5) + 1 for i in range(40)]),
+                                              (128, 2, [70], 40), (64, 32, [9], [1, 700, 1, 1, 65, 64, 63, 300, 2]), (128, 8, [3], 900)])
+def test_shared_attention_of_single_members_keys(d, hq, members, own):
+    c = Shared(members, [150, 90][:len(members)], own, hq=hq, hkv=1, d=d, dtype=torch.bfloat16, seed=17).device()
+    c.call()
+    c.check()
+
+
+def test_shared_attention_of_very_many_small_groups():
+    """More pieces than a block lists at a time."""
+    n = 1700
+    c = Shared([1] * n, [5 + i % 3 for i in range(n)], [1 + i % 4 for i in range(n)], hq=4, hkv=4, d=64, dtype=torch.bfloat16, seed=16).device()
     c.call()
     c.check()
 

@@ -296,11 +296,42 @@ static int launch_merge(const SharedParams& p, cudaStream_t stream) {
 // Whether the kernels of attention_shared_tc.cu take a shape (addresses on 16 bytes besides).
 TK_API int tk_attention_shared_tc_takes(int n_q_heads, int n_kv_heads, int head_dim, int v_dim, int page_size) {
   tk::SharedParams p = {};
-  p.n_q_heads = n_q_heads; p.n_kv_heads = n_kv_heads; p.d = head_dim; p.dv = v_dim; p.page_size = page_size;
+  p.n_q_heads = n_q_heads; p.n_kv_heads = n_kv_heads; p.d = head_dim; p.dv = v_dim; p.page_size = page_size; p.n_own = 1;
   return tk::shared_tc_takes(p);
 }
 
-// scratch: rows * n_q_heads * (n_shared + n_own) * (dv + 2) floats on 16 bytes, with an odd v_dim one more.
+// scratch: 16-byte aligned, as many floats as tk_attention_shared_scratch says for the same arguments.
+static int shared_params(tk::SharedParams& p, const void* q, void* out, const void* k_cache, const void* v_cache, int n_rows, int n_groups,
+                         int max_members, int n_q_heads, int n_kv_heads, int head_dim, int v_dim, int page_size, int num_pages, int n_shared,
+                         int n_own, const unsigned char* history, int dtype) {
+  const long long parts = (long long)n_rows * n_q_heads * ((long long)n_shared + n_own);
+  if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads != 0 || head_dim < 1 || head_dim > 256 || v_dim < 1 || v_dim > 256 ||
+      page_size < 1 || max_members < 1 || n_shared < 0 || n_own < 1 || parts > 0x7fffffffLL || (dtype != tk::kF32 && dtype != tk::kBF16)) {
+    return (int)cudaErrorInvalidValue;
+  }
+  p = {};
+  p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.history = history;
+  p.n_rows = n_rows; p.n_groups = n_groups; p.max_members = max_members; p.n_q_heads = n_q_heads; p.n_kv_heads = n_kv_heads;
+  p.d = head_dim; p.dv = v_dim; p.page_size = page_size; p.num_pages = num_pages;
+  p.n_shared = n_shared; p.n_own = n_own; p.n_parts = n_shared + n_own;
+  return 0;
+}
+
+static bool on_tensor_cores(const tk::SharedParams& p, int dtype) { return dtype == tk::kBF16 && tk::shared_tc_takes(p); }
+
+TK_API long long tk_attention_shared_scratch(const void* q, void* out, const void* k_cache, const void* v_cache, const unsigned char* history,
+                                             int n_rows, int n_groups, int max_members, int n_q_heads, int n_kv_heads, int head_dim, int v_dim,
+                                             int page_size, int num_pages, int n_shared, int n_own, int dtype) {
+  tk::SharedParams p;
+  if (shared_params(p, q, out, k_cache, v_cache, n_rows, n_groups, max_members, n_q_heads, n_kv_heads, head_dim, v_dim, page_size, num_pages,
+                    n_shared, n_own, history, dtype) != 0) {
+    return -1;
+  }
+  if (on_tensor_cores(p, dtype)) return tk::shared_tc_scratch(p, tk::device_sm_count());
+  const long long parts = (long long)n_rows * n_q_heads * p.n_parts;
+  return (parts * v_dim + 1) / 2 * 2 + 2 * parts;
+}
+
 TK_API int tk_attention_shared(const void* q, void* out, const void* k_cache, const void* v_cache, const int* group_start,
                                const int* prefix_slot, const int* prefix_len, const int* positions, const int* req_slot,
                                const int* block_table, const unsigned char* history, const float* sinks, float* scratch,
@@ -309,33 +340,25 @@ TK_API int tk_attention_shared(const void* q, void* out, const void* k_cache, co
                                int window, int n_shared, int n_own, float scale, float softcap, int dtype,
                                cudaStream_t stream) {
   if (n_rows <= 0 || n_groups <= 0) return 0;
-  const long long parts = (long long)n_rows * n_q_heads * ((long long)n_shared + n_own);
-  if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads != 0 || head_dim < 1 || head_dim > 256 || v_dim < 1 || v_dim > 256 ||
-      page_size < 1 || max_members < 1 || n_shared < 0 || n_own < 1 || max_slots < 1 || max_pages < 1 ||
-      parts > 0x7fffffffLL || (history != nullptr && history_ld < 1)) {
-    return (int)cudaErrorInvalidValue;
-  }
   tk::SharedParams p;
-  p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.group_start = group_start; p.prefix_slot = prefix_slot;
-  p.prefix_len = prefix_len; p.positions = positions; p.req_slot = req_slot; p.block_table = block_table; p.history = history;
-  p.sinks = sinks; p.err = err;
-  p.n_rows = n_rows; p.n_groups = n_groups; p.max_members = max_members; p.n_q_heads = n_q_heads; p.n_kv_heads = n_kv_heads;
-  p.d = head_dim; p.dv = v_dim; p.page_size = page_size; p.max_pages = max_pages; p.num_pages = num_pages;
-  p.max_slots = max_slots; p.history_ld = history_ld; p.window = window;
-  p.n_shared = n_shared; p.n_own = n_own; p.n_parts = n_shared + n_own;
-  p.part_o = scratch;
-  p.part_ml = scratch + (parts * v_dim + 1) / 2 * 2;
+  const int bad = shared_params(p, q, out, k_cache, v_cache, n_rows, n_groups, max_members, n_q_heads, n_kv_heads, head_dim, v_dim, page_size,
+                                num_pages, n_shared, n_own, history, dtype);
+  if (bad != 0) return bad;
+  if (max_slots < 1 || max_pages < 1 || (history != nullptr && history_ld < 1) || ((uintptr_t)scratch & 15) != 0) return (int)cudaErrorInvalidValue;
+  p.group_start = group_start; p.prefix_slot = prefix_slot; p.prefix_len = prefix_len; p.positions = positions; p.req_slot = req_slot;
+  p.block_table = block_table; p.sinks = sinks; p.err = err; p.scratch = scratch;
+  p.max_pages = max_pages; p.max_slots = max_slots; p.history_ld = history_ld; p.window = window;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.cap_log2 = softcap > 0.0f ? softcap * 1.4426950408889634f : 0.0f;
   p.inv_cap = softcap > 0.0f ? scale / softcap : 0.0f;
+  if (on_tensor_cores(p, dtype)) return tk::launch_shared_tc(p, tk::device_sm_count(), stream);
+  const long long parts = (long long)n_rows * n_q_heads * p.n_parts;
+  p.part_o = scratch;
+  p.part_ml = scratch + (parts * v_dim + 1) / 2 * 2;
   const uintptr_t mask = dtype == tk::kF32 ? 15 : 7;
   p.wide_k = head_dim % 4 == 0 && (((uintptr_t)q | (uintptr_t)k_cache) & mask) == 0;
   p.wide_v = v_dim % 4 == 0 && ((uintptr_t)v_cache & mask) == 0;
-  if (dtype == tk::kF32) {
-    const int e = tk::launch_general<float>(p, stream);
-    return e != 0 ? e : tk::launch_merge<float>(p, stream);
-  }
-  if (dtype != tk::kBF16) return (int)cudaErrorInvalidValue;
-  const int e = tk::shared_tc_takes(p) ? tk::launch_shared_tc(p, stream) : tk::launch_general<__nv_bfloat16>(p, stream);
-  return e != 0 ? e : tk::launch_merge<__nv_bfloat16>(p, stream);
+  const int e = dtype == tk::kF32 ? tk::launch_general<float>(p, stream) : tk::launch_general<__nv_bfloat16>(p, stream);
+  if (e != 0) return e;
+  return dtype == tk::kF32 ? tk::launch_merge<float>(p, stream) : tk::launch_merge<__nv_bfloat16>(p, stream);
 }

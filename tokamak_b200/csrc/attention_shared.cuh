@@ -32,8 +32,9 @@ struct SharedParams {
   const int* block_table;       // [max_slots, max_pages]
   const unsigned char* history; // [max_slots, history_ld] or null
   const float* sinks;           // [n_q_heads] or null
-  float* part_o;                // [rows, n_q_heads, n_parts, dv]
+  float* part_o;                // [rows, n_q_heads, n_parts, dv]   (the general kernel's)
   float* part_ml;               // [rows, n_q_heads, n_parts, 2]
+  float* scratch;               // 16-byte aligned
   int* err;
   int n_rows, n_groups, max_members, n_q_heads, n_kv_heads, d, dv, page_size, max_pages, num_pages, max_slots, history_ld, window;
   int n_shared, n_own, n_parts; // parts of the shared and of the other positions; n_parts = n_shared + n_own
@@ -106,8 +107,9 @@ __device__ __forceinline__ RowSpan row_span(const SharedParams& p, int row) {
 }
 
 // ---- attention_shared_tc.cu -------------------------------------------------------------------------------------------
-// bfloat16 heads of 64 or 128: the shared positions on tcgen05, the others on mma.sync; parts as the general kernel's.
+// bfloat16 heads of 64 or 128: the shared positions on tcgen05, the others on mma.sync.
 bool shared_tc_takes(const SharedParams& p);
-int launch_shared_tc(const SharedParams& p, cudaStream_t stream);
+long long shared_tc_scratch(const SharedParams& p, int sms);
+int launch_shared_tc(const SharedParams& p, int sms, cudaStream_t stream);
 
 }  // namespace tk

@@ -167,7 +167,8 @@ def library() -> ctypes.CDLL:
         fn.argtypes = argtypes
         fn.restype = c_int
     for name, args in (("tk_gemm_chain_scratch_floats", [c_int]), ("tk_gemm_chain_counter_ints", [c_int]),
-                       ("tk_attention_decode_balanced_scratch_floats", [c_int, c_int])):
+                       ("tk_attention_decode_balanced_scratch_floats", [c_int, c_int]),
+                       ("tk_attention_shared_scratch", 5 * [_P] + 12 * [c_int])):
         fn = getattr(lib, name)
         fn.argtypes = args
         fn.restype = c_longlong

@@ -1992,24 +1992,17 @@ def shared_tc_takes(n_q_heads: int, n_kv_heads: int, head_dim: int, v_dim: int, 
     return bool(library().tk_attention_shared_tc_takes(n_q_heads, n_kv_heads, head_dim, v_dim, page_size))
 
 
-def shared_splits(device: torch.device, groups: int, rows: int, n_q_heads: int, n_kv_heads: int, shared: SharedPrefix,
+def shared_splits(sms: int, groups: int, rows: int, n_q_heads: int, n_kv_heads: int, shared: SharedPrefix,
                   window: int | None, tensor_cores: bool) -> tuple[int, int]:
-    """Parts that the shared and the other positions are cut into.  The tensor-core kernel of the shared ones has a block per
-    SM and 128 or 256 (query head, member) pairs in each; all other blocks are small and several to an SM."""
-    sms = sm_count(device)
-    per = n_q_heads // n_kv_heads
+    """Parts that the shared and the other positions are cut into: enough small blocks for two an SM, none with less than 64
+    keys.  The tensor-core kernel deals its work out itself; what counts for it is whether anything is shared."""
     keys = min(shared.max_prefix, window or shared.max_prefix)
     if tensor_cores:
-        tile = 128 // per
-        tile *= 2 if shared.max_members > tile else 1
-        fill, least = sms, 128
-    else:
-        tile, fill, least = 32 / per, 2 * sms, 64
-    blocks = groups * n_kv_heads * math.ceil(shared.max_members / tile)
-    n_shared = max(1, min(fill // blocks, -(-keys // least))) if keys > 0 else 0
+        return int(keys > 0), 1
     own = min(shared.max_own, window or shared.max_own)
-    n_own = max(1, min(2 * sms // max(1, rows * n_kv_heads), -(-own // least)))
-    return n_shared, n_own
+    blocks = groups * n_kv_heads * -(-shared.max_members * (n_q_heads // n_kv_heads) // 32)
+    n_shared = max(1, min(2 * sms // max(1, blocks), -(-keys // 64))) if keys > 0 else 0
+    return n_shared, max(1, min(2 * sms // max(1, rows * n_kv_heads), -(-own // 64)))
 
 
 def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, shared: SharedPrefix,
@@ -2064,14 +2057,18 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     if rows == 0:
         return
     tensor_cores = dtype == 1 and shared_tc_takes(hq, hkv, d, dv, page_size)
-    n_shared, n_own = shared_splits(q.device, groups, rows, hq, hkv, shared, window, tensor_cores)
-    scratch = torch.empty(rows * hq * (n_shared + n_own) * (dv + 2) + 1, dtype=torch.float32, device=q.device)
-    _check(_lib().tk_attention_shared(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                      shared.group_start.data_ptr(), shared.prefix_slot.data_ptr(), shared.prefix_len.data_ptr(),
-                                      positions.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), _ptr(history), _ptr(sinks),
-                                      scratch.data_ptr(), err.data_ptr(), rows, groups, shared.max_members, hq, hkv, d, dv,
-                                      page_size, block_table.shape[1], num_pages, block_table.shape[0], ld, int(window or 0),
-                                      n_shared, n_own, float(scale), float(softcap or 0.0), dtype, _stream()),
+    n_shared, n_own = shared_splits(sm_count(q.device), groups, rows, hq, hkv, shared, window, tensor_cores)
+    lib = _lib()
+    sizes = (rows, groups, shared.max_members, hq, hkv, d, dv, page_size)
+    ptrs = (q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr())
+    need = lib.tk_attention_shared_scratch(*ptrs, _ptr(history), *sizes, num_pages, n_shared, n_own, dtype)
+    if need < 0:
+        raise KernelError(f"the shared-prefix attention does not take {rows} rows of {hq} heads in {n_shared} + {n_own} parts")
+    scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+    _check(lib.tk_attention_shared(*ptrs, shared.group_start.data_ptr(), shared.prefix_slot.data_ptr(), shared.prefix_len.data_ptr(),
+                                   positions.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), _ptr(history), _ptr(sinks),
+                                   scratch.data_ptr(), err.data_ptr(), *sizes, block_table.shape[1], num_pages, block_table.shape[0], ld,
+                                   int(window or 0), n_shared, n_own, float(scale), float(softcap or 0.0), dtype, _stream()),
            "attention_shared")
 
 
