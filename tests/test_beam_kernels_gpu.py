@@ -550,6 +550,20 @@ def test_shared_attention_of_very_many_small_groups():
     c.check()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_shared_attention_of_keys_that_come_late(d):
+    """Long sequences of key tiles in every block, read from memory that no cache holds: what a tile waits for arrives late."""
+    x = Shared([2] * 12, [1180 + 49 * i for i in range(12)], own=40, hq=16, hkv=8, d=d, history=True, common=30, seed=5).device()
+    first = x.call().clone()
+    x.check(first)
+    cold = torch.empty(1 << 28, dtype=torch.uint8, device=DEV)
+    for i in range(24):
+        cold.fill_(i)
+        x.out.fill_(float("nan"))
+        assert torch.equal(x.call(), first), f"call {i}"
+    x.check()
+
+
 def test_shared_attention_at_addresses_on_any_boundary():
     for dtype in (torch.float32, torch.bfloat16):
         c = Shared([3], [70], 20, d=64, dtype=dtype, seed=13).device()

@@ -565,8 +565,12 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           const int key_first = prefix ? (x.lo_tile + x.tile0 + j) * kSpBN : x.common0 + (x.tile0 + j - x.prefix_tiles) * kSpBN;
           const int last = prefix ? x.hi : x.common1 - 1;
           const int hi_r = min(last, sp.pos), lo_r = sp.lo;          // a row without a position sees nothing
+          ok = __all_sync(0xffffffffu, mbar_wait(s_full(t, bf), (g >> 1) & 1u, abort_flag));
+          if (!ok) { if (lane == 0) { set_error(p.err, kErrWait, 43, j, t); *abort_flag = 1; } break; }
           if (prefix && quarter == 0 && (key_first < x.lo || key_first + kSpBN - 1 > x.hi)) {
-            // values that nobody sees (each group for itself, where both read them: their products are not ordered)
+            // Values that nobody sees (each group for itself, where both read them: their products are not ordered).  Not before
+            // the scores: they say that the values this stage held before have been seen by the group's issuer, without which
+            // the wait below could take an older filling, that has yet to arrive, for this one.
             ok = __all_sync(0xffffffffu, mbar_wait(gt_smem_u32(&v_full[st]), ph, abort_flag));
             if (!ok) { if (lane == 0) { set_error(p.err, kErrWait, 42, j, t); *abort_flag = 1; } break; }
             unsigned char* v = smem + 2 * Q_BYTES + V_RING + st * KV_BYTES;
@@ -578,8 +582,6 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             }
             fence_async_shared();
           }
-          ok = __all_sync(0xffffffffu, mbar_wait(s_full(t, bf), (g >> 1) & 1u, abort_flag));
-          if (!ok) { if (lane == 0) { set_error(p.err, kErrWait, 43, j, t); *abort_flag = 1; } break; }
           if (active) {
             tc_fence_after();
             uint32_t sraw[kSpBN];
