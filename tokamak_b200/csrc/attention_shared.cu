@@ -33,7 +33,7 @@ __device__ __forceinline__ void load_row(float* dst, const T* src, int n, bool w
 }
 
 template <typename T, int kChunks>       // kChunks: 128-column chunks of a value row
-__global__ void __launch_bounds__(kShThreads) shared_parts_kernel(SharedParams p, int row_tiles, int n_shared_blocks) {
+__global__ void __launch_bounds__(kShThreads) shared_parts_kernel(SharedParams p, int shared_tiles, int own_tiles, int n_shared_blocks) {
   pdl_trigger();
   extern __shared__ __align__(16) float s_mem[];
   __shared__ long long s_row[kShKeys];
@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(kShThreads) shared_parts_kernel(SharedParams p
   const int splits = shared ? p.n_shared : p.n_own;
   const int split = b % splits; b /= splits;
   const int hkv = b % p.n_kv_heads; b /= p.n_kv_heads;
+  const int row_tiles = shared ? shared_tiles : own_tiles;
   const int tile = b % row_tiles; b /= row_tiles;
   int g, first_pair, n_pairs, prefix, slot = -1, own_row = -1;
   int2 rows;
@@ -241,16 +242,26 @@ __global__ void __launch_bounds__(kMergeWarps * 32) shared_merge_kernel(SharedPa
       const float f = mine.y > 0.0f ? exp2f(mine.x - m_all) : 0.0f;
       l_all += f * mine.y;
       const int n = min(32, p.n_parts - i0);
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float w = __shfl_sync(0xffffffffu, f, i);
-        if (w == 0.0f || c >= p.dv) continue;        // an empty part has no output that is anything
-        const float* src = o + (size_t)(i0 + i) * p.dv + c;
-        if (wide) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-          acc[0] += v.x * w; acc[1] += v.y * w; acc[2] += v.z * w; acc[3] += v.w * w;
-        } else {
-          for (int e = 0; e < 4 && c + e < p.dv; ++e) acc[e] += __ldcg(src + e) * w;
+      // eight parts' loads at a time: they have nothing to wait for but each other's latency
+      for (int j = 0; j < n; j += 8) {
+        float v[8][4], w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          w[k] = j + k < n ? __shfl_sync(0xffffffffu, f, j + k) : 0.0f;
+          v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.0f;
+          if (w[k] == 0.0f || c >= p.dv) continue;        // an empty part has no output that is anything
+          const float* src = o + (size_t)(i0 + j + k) * p.dv + c;
+          if (wide) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+            v[k][0] = x.x; v[k][1] = x.y; v[k][2] = x.z; v[k][3] = x.w;
+          } else {
+            for (int e = 0; e < 4 && c + e < p.dv; ++e) v[k][e] = __ldcg(src + e);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] += v[k][e] * w[k];
         }
       }
     }
@@ -271,15 +282,11 @@ static int launch_general(const SharedParams& p, cudaStream_t stream) {
   const int shared_tiles = (p.max_members * per + kShRows - 1) / kShRows, own_tiles = (per + kShRows - 1) / kShRows;
   const long long n_shared = (long long)p.n_groups * shared_tiles * p.n_kv_heads * p.n_shared;
   const long long n_own = (long long)p.n_rows * own_tiles * p.n_kv_heads * p.n_own;
-  if (n_shared > 0x7fffffffLL || n_own > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+  if (n_shared + n_own > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   auto run = [&](auto kernel) -> int {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    if (n_shared > 0) {
-      e = launch(kernel, dim3((unsigned)n_shared), dim3(kShThreads), smem, stream, p, shared_tiles, (int)n_shared);
-      if (e != cudaSuccess) return (int)e;
-    }
-    return (int)launch(kernel, dim3((unsigned)n_own), dim3(kShThreads), smem, stream, p, own_tiles, 0);
+    return (int)launch(kernel, dim3((unsigned)(n_shared + n_own)), dim3(kShThreads), smem, stream, p, shared_tiles, own_tiles, (int)n_shared);
   };
   return p.dv <= 128 ? run(shared_parts_kernel<T, 1>) : run(shared_parts_kernel<T, 2>);
 }

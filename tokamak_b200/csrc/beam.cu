@@ -595,7 +595,12 @@ __global__ void __launch_bounds__(64) beam_advance_kernel(AdvanceParams p) {
 // place.  A thread owns a column of 16 bytes (less where the records' size or address asks for it) of all records of one
 // group: it reads every source that moves, then writes, so no order of the moves can go wrong and no copy is made.  Bound by
 // the bytes: sources that move are read, seats that change are written, nothing else is touched.
+// Before its first load a block has to know which seats change, which costs it as long as a column's loads: where there are more
+// columns than threads at a time on the device, a thread takes up to four, one after the other.  12 groups of 8 beams with 8
+// layers of 1 MB states, 313 MB to read and write: 66 us (4.7 TB/s) against 87 with a column each, 72 with two, 64 to 68
+// with eight or sixteen, which cost a call of 60 MB 14.3 us instead of 12.8.
 constexpr int kMoveThreads = 256;
+constexpr int kMoveColumns = 4;
 constexpr int kMoveMaxTensors = 24;
 constexpr int kMoveMaxSeats = 64;
 
@@ -611,22 +616,28 @@ struct MoveParams {
   const int* parents;           // [groups, seats]
   int* err;
   int n_tensors, seats, max_slots;
+  int per_thread;               // columns of a thread
 };
 
 template <typename V, int kSeats>
-__device__ __forceinline__ void move_column(const MoveTensor& t, long long at, const int* s_src, const int* s_dst, int n, int max_slots) {
-  const long long columns = t.bytes / (long long)sizeof(V);
-  if (at >= columns * t.keys) return;
-  const long long key = at / columns, col = at % columns;
-  V* base = reinterpret_cast<V*>(t.base) + key * max_slots * columns + col;
-  V v[kSeats];
+__device__ __forceinline__ void move_columns(const MoveTensor& t, long long first, int count, const int* s_src, const int* s_dst, int n,
+                                             int max_slots) {
+  const long long columns = t.bytes / (long long)sizeof(V), all = columns * t.keys;
+#pragma unroll 1
+  for (int c = 0; c < count; ++c, first += kMoveThreads) {
+    const long long at = first + threadIdx.x;
+    if (at >= all) return;
+    const long long key = all <= 0x7fffffffLL ? (long long)((unsigned)at / (unsigned)columns) : at / columns;
+    V* base = reinterpret_cast<V*>(t.base) + key * (max_slots - 1) * columns + at;          // column at % columns of the key's records
+    V v[kSeats];
 #pragma unroll
-  for (int i = 0; i < kSeats; ++i) {
-    if (i < n) v[i] = base[(long long)s_src[i] * columns];
-  }
+    for (int i = 0; i < kSeats; ++i) {
+      if (i < n) v[i] = base[(long long)s_src[i] * columns];
+    }
 #pragma unroll
-  for (int i = 0; i < kSeats; ++i) {
-    if (i < n) base[(long long)s_dst[i] * columns] = v[i];
+    for (int i = 0; i < kSeats; ++i) {
+      if (i < n) base[(long long)s_dst[i] * columns] = v[i];
+    }
   }
 }
 
@@ -639,18 +650,23 @@ __global__ void __launch_bounds__(kMoveThreads) reorder_slots_kernel(const __gri
   const int g = blockIdx.y;
   if (threadIdx.x < 32) {
     // the seats that change, in order
+    const int lane = threadIdx.x;
+    const int* slots = p.slots + (size_t)g * p.seats;
+    const int* parents = p.parents + (size_t)g * p.seats;
+    const int slot0 = lane < p.seats ? slots[lane] : -1, slot1 = lane + 32 < p.seats ? slots[lane + 32] : -1;
+    const int parent0 = lane < p.seats ? parents[lane] : 0, parent1 = lane + 32 < p.seats ? parents[lane + 32] : 0;
     int n = 0;
-    for (int i0 = 0; i0 < p.seats; i0 += 32) {
-      const int i = i0 + (int)threadIdx.x;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = lane + 32 * h;
+      const int parent = h == 0 ? parent0 : parent1, dst = h == 0 ? slot0 : slot1;
+      const int low = __shfl_sync(0xffffffffu, slot0, parent & 31), high = __shfl_sync(0xffffffffu, slot1, parent & 31);
+      const int src = parent < 32 ? low : high;
       bool moves = false;
-      int src = 0, dst = 0;
       if (i < p.seats) {
-        const int parent = p.parents[(size_t)g * p.seats + i];
-        dst = p.slots[(size_t)g * p.seats + i];
         if (parent < 0 || parent >= p.seats) {
           set_error(p.err, kErrRequest, g, parent, p.seats);
         } else if (parent != i) {
-          src = p.slots[(size_t)g * p.seats + parent];
           if (src < 0 || src >= p.max_slots || dst < 0 || dst >= p.max_slots) {
             set_error(p.err, kErrRequest, g, src < 0 || src >= p.max_slots ? src : dst, p.max_slots);
           } else {
@@ -660,13 +676,13 @@ __global__ void __launch_bounds__(kMoveThreads) reorder_slots_kernel(const __gri
       }
       const unsigned mask = __ballot_sync(0xffffffffu, moves);
       if (moves) {
-        const int at = n + __popc(mask & ((1u << threadIdx.x) - 1u));
+        const int at = n + __popc(mask & ((1u << lane) - 1u));
         s_src[at] = src;
         s_dst[at] = dst;
       }
       n += __popc(mask);
     }
-    if (threadIdx.x == 0) s_n = n;
+    if (lane == 0) s_n = n;
   }
   __syncthreads();
   const int n = s_n;
@@ -674,12 +690,12 @@ __global__ void __launch_bounds__(kMoveThreads) reorder_slots_kernel(const __gri
   int k = 0;
   while (k + 1 < p.n_tensors && (long long)blockIdx.x >= p.t[k + 1].first_block) ++k;
   const MoveTensor& t = p.t[k];
-  const long long at = ((long long)blockIdx.x - t.first_block) * kMoveThreads + threadIdx.x;
-  if (kSeats <= 32 && t.vec == 16) move_column<uint4, (kSeats <= 32 ? kSeats : 1)>(t, at, s_src, s_dst, n, p.max_slots);
-  else if (t.vec == 8) move_column<uint2, kSeats>(t, at, s_src, s_dst, n, p.max_slots);
-  else if (t.vec == 4) move_column<unsigned int, kSeats>(t, at, s_src, s_dst, n, p.max_slots);
-  else if (t.vec == 2) move_column<unsigned short, kSeats>(t, at, s_src, s_dst, n, p.max_slots);
-  else move_column<unsigned char, kSeats>(t, at, s_src, s_dst, n, p.max_slots);
+  const long long at = ((long long)blockIdx.x - t.first_block) * kMoveThreads * p.per_thread;
+  if (kSeats <= 32 && t.vec == 16) move_columns<uint4, (kSeats <= 32 ? kSeats : 1)>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
+  else if (t.vec == 8) move_columns<uint2, kSeats>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
+  else if (t.vec == 4) move_columns<unsigned int, kSeats>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
+  else if (t.vec == 2) move_columns<unsigned short, kSeats>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
+  else move_columns<unsigned char, kSeats>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
 }
 
 }  // namespace tk
@@ -744,7 +760,7 @@ TK_API int tk_reorder_slots(void* const* bases, const long long* bytes, const in
   }
   tk::MoveParams p;
   p.slots = slots; p.parents = parents; p.err = err; p.n_tensors = 0; p.seats = seats; p.max_slots = max_slots;
-  long long blocks = 0;
+  long long columns = 0;
   for (int i = 0; i < n_tensors; ++i) {
     if (bytes[i] < 0 || keys[i] < 0) return (int)cudaErrorInvalidValue;
     if (bytes[i] == 0 || keys[i] == 0) continue;
@@ -756,8 +772,16 @@ TK_API int tk_reorder_slots(void* const* bases, const long long* bytes, const in
     // 64 seats of 16 bytes would not fit a thread's registers
     if (seats > 32) t.vec = 8;
     while (((uintptr_t)bases[i] | (unsigned long long)bytes[i]) % (unsigned long long)t.vec) t.vec /= 2;
+    columns += t.bytes / t.vec * t.keys;
+  }
+  p.per_thread = 1;
+  while (p.per_thread < tk::kMoveColumns && columns * groups > 8LL * tk::device_sm_count() * tk::kMoveThreads * p.per_thread) p.per_thread *= 2;
+  long long blocks = 0;
+  for (int i = 0; i < p.n_tensors; ++i) {
+    tk::MoveTensor& t = p.t[i];
+    const long long per_block = (long long)tk::kMoveThreads * p.per_thread;
     t.first_block = blocks;
-    blocks += (t.bytes / t.vec * t.keys + tk::kMoveThreads - 1) / tk::kMoveThreads;
+    blocks += (t.bytes / t.vec * t.keys + per_block - 1) / per_block;
   }
   if (blocks == 0) return 0;
   if (blocks > 0x7fffffffLL) return (int)cudaErrorInvalidValue;

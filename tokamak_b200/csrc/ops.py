@@ -1994,15 +1994,15 @@ def shared_tc_takes(n_q_heads: int, n_kv_heads: int, head_dim: int, v_dim: int, 
 
 def shared_splits(sms: int, groups: int, rows: int, n_q_heads: int, n_kv_heads: int, shared: SharedPrefix,
                   window: int | None, tensor_cores: bool) -> tuple[int, int]:
-    """Parts that the shared and the other positions are cut into: enough small blocks for two an SM, none with less than 64
+    """Parts that the shared and the other positions are cut into: enough small blocks for two an SM, none with less than 32
     keys.  The tensor-core kernel deals its work out itself; what counts for it is whether anything is shared."""
     keys = min(shared.max_prefix, window or shared.max_prefix)
     if tensor_cores:
         return int(keys > 0), 1
     own = min(shared.max_own, window or shared.max_own)
     blocks = groups * n_kv_heads * -(-shared.max_members * (n_q_heads // n_kv_heads) // 32)
-    n_shared = max(1, min(2 * sms // max(1, blocks), -(-keys // 64))) if keys > 0 else 0
-    return n_shared, max(1, min(2 * sms // max(1, rows * n_kv_heads), -(-own // 64)))
+    n_shared = max(1, min(2 * sms // max(1, blocks), -(-keys // 32))) if keys > 0 else 0
+    return n_shared, max(1, min(2 * sms // max(1, rows * n_kv_heads), -(-own // 32)))
 
 
 def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, shared: SharedPrefix,
