@@ -751,9 +751,9 @@ TK_API int tk_beam_advance(const float* cand_scores, const int* cand_parents, co
   return (int)tk::launch(tk::beam_advance_kernel, dim3(groups), dim3(64), 0, stream, p);
 }
 
-// bases, bytes, keys: of every tensor; a record's bytes and its tensor's address decide how wide its columns are.
-TK_API int tk_reorder_slots(void* const* bases, const long long* bytes, const int* keys, int n_tensors, const int* slots,
-                            const int* parents, int* err, int groups, int seats, int max_slots, cudaStream_t stream) {
+// tensors: address, bytes of a record and keys of each; a record's bytes and its tensor's address decide how wide its columns are.
+TK_API int tk_reorder_slots(const long long* tensors, int n_tensors, const int* slots, const int* parents, int* err, int groups,
+                            int seats, int max_slots, cudaStream_t stream) {
   if (groups <= 0 || n_tensors <= 0) return 0;
   if (n_tensors > tk::kMoveMaxTensors || seats < 1 || seats > tk::kMoveMaxSeats || groups > 65535 || max_slots < 1) {
     return (int)cudaErrorInvalidValue;
@@ -762,16 +762,17 @@ TK_API int tk_reorder_slots(void* const* bases, const long long* bytes, const in
   p.slots = slots; p.parents = parents; p.err = err; p.n_tensors = 0; p.seats = seats; p.max_slots = max_slots;
   long long columns = 0;
   for (int i = 0; i < n_tensors; ++i) {
-    if (bytes[i] < 0 || keys[i] < 0) return (int)cudaErrorInvalidValue;
-    if (bytes[i] == 0 || keys[i] == 0) continue;
+    const long long base = tensors[3 * i], bytes = tensors[3 * i + 1], keys = tensors[3 * i + 2];
+    if (bytes < 0 || keys < 0 || keys > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+    if (bytes == 0 || keys == 0) continue;
     tk::MoveTensor& t = p.t[p.n_tensors++];
-    t.base = (unsigned char*)bases[i];
-    t.bytes = bytes[i];
-    t.keys = keys[i];
+    t.base = (unsigned char*)base;
+    t.bytes = bytes;
+    t.keys = (int)keys;
     t.vec = 16;
     // 64 seats of 16 bytes would not fit a thread's registers
     if (seats > 32) t.vec = 8;
-    while (((uintptr_t)bases[i] | (unsigned long long)bytes[i]) % (unsigned long long)t.vec) t.vec /= 2;
+    while (((unsigned long long)base | (unsigned long long)bytes) % (unsigned long long)t.vec) t.vec /= 2;
     columns += t.bytes / t.vec * t.keys;
   }
   p.per_thread = 1;

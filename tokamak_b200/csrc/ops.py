@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+from array import array
 from dataclasses import dataclass
 from functools import lru_cache
 
@@ -222,11 +223,13 @@ def sample_slots(logits: torch.Tensor, records: torch.Tensor, row_slot: torch.Te
                                      err.data_ptr(), _stream()), "sample_slots")
 
 
-def _want_here(**tensors) -> None:
-    """Refuses tensors of a device other than the current one: the launch goes to the current device's stream."""
+def _want_here(*wants) -> None:
+    """:func:`_want` for ``(tensor, type, name)``, of which none may be on a device other than the current one: the launch goes to
+    the current device's stream."""
     here = _raw_device()
-    for name, t in tensors.items():
-        if t is not None and t.get_device() != here:
+    for t, dtype, name in wants:
+        if t.get_device() != here or t.dtype != dtype or not t.is_contiguous():
+            _want(t, dtype, name)
             raise KernelError(f"{name} must be on the current CUDA device {here}, it is on {t.device}")
 
 
@@ -259,7 +262,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int, *, 
     logits of -inf or NaN.  ``out``: tensors to write to."""
     if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
         raise KernelError("logits must be a float32 CUDA tensor [groups * beams, vocab] whose rows are contiguous")
-    _want(scores, torch.float32, "scores")
+    if logits.get_device() != _raw_device():
+        raise KernelError(f"logits must be on the current CUDA device {_raw_device()}, they are on {logits.device}")
     if scores.dim() != 2:
         raise KernelError(f"scores must be [groups, beams], got shape {tuple(scores.shape)}")
     groups, beams = scores.shape
@@ -280,11 +284,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int, *, 
         out = (torch.empty(shape, dtype=torch.float32, device=logits.device),
                torch.empty(shape, dtype=torch.int32, device=logits.device),
                torch.empty(shape, dtype=torch.int32, device=logits.device))
-    for name, t, dtype in zip(("scores", "parents", "tokens"), out, (torch.float32, torch.int32, torch.int32)):
-        _want(t, dtype, "out " + name)
+    _want_here((scores, torch.float32, "scores"), (out[0], torch.float32, "out scores"), (out[1], torch.int32, "out parents"),
+               (out[2], torch.int32, "out tokens"))
+    for t in out:
         if t.shape != shape:
-            raise KernelError(f"out {name} must be {shape}, got {tuple(t.shape)}")
-    _want_here(logits=logits, scores=scores, out=out[0], parents=out[1], tokens=out[2])
+            raise KernelError(f"the three tensors of out must be {shape}, got {tuple(t.shape)}")
     if groups == 0:
         return out
     segments = beam_segments(sm_count(logits.device), rows, beams, vocab, candidates)
@@ -309,44 +313,40 @@ def beam_advance(candidates: tuple, stop_tokens: torch.Tensor | None, slots: tor
     beams]``) receives the token.  ``history`` (uint8 ``[slots, n]``): the place ``positions - prefix_len`` of each
     seat's row receives the seat (see :class:`SharedPrefix`); call :func:`reorder_slots` afterwards.  ``begin``: the candidates
     continue one row (a search that begins); every seat goes on from itself, and the history is left alone."""
-    for name, t, dtype in (("candidate scores", candidates[0], torch.float32), ("candidate parents", candidates[1], torch.int32),
-                           ("candidate tokens", candidates[2], torch.int32)):
-        _want(t, dtype, name)
+    _want_here((candidates[0], torch.float32, "candidate scores"), (candidates[1], torch.int32, "candidate parents"),
+               (candidates[2], torch.int32, "candidate tokens"), (slots, torch.int32, "slots"), (scores, torch.float32, "scores"),
+               (parents, torch.int32, "parents"), (tokens, torch.int32, "tokens"), (err, torch.int32, "err"))
+    for t in candidates:
         if t.dim() != 2 or t.shape != candidates[0].shape:
             raise KernelError("the candidates must be three tensors [groups, candidates]")
     groups, k = candidates[0].shape
-    for name, t, dtype in (("slots", slots, torch.int32), ("scores", scores, torch.float32), ("parents", parents, torch.int32),
-                           ("tokens", tokens, torch.int32)):
-        _want(t, dtype, name)
+    for name, t in (("slots", slots), ("scores", scores), ("parents", parents), ("tokens", tokens)):
         if t.dim() != 2 or t.shape != slots.shape or t.shape[0] != groups:
             raise KernelError(f"{name} must be [groups, beams] for {groups} groups, got {tuple(t.shape)}")
     beams = slots.shape[1]
     if not 1 <= beams <= BEAM_MAX or k < 1:
         raise KernelError(f"a group has 1 to {BEAM_MAX} beams and a candidate at least, got {beams} and {k}")
-    _want(err, torch.int32, "err")
     n_stop = 0
     if stop_tokens is not None:
-        _want(stop_tokens, torch.int32, "stop_tokens")
+        _want_here((stop_tokens, torch.int32, "stop_tokens"))
         n_stop = stop_tokens.numel()
     max_slots, words, ld = 1 << 30, 0, 0
     if records is not None:
-        _want(records, torch.int32, "records")
+        _want_here((records, torch.int32, "records"))
         if records.dim() != 2 or not 0 <= token_word < records.shape[1]:
             raise KernelError(f"records must be [slots, words] with a word {token_word}, got {tuple(records.shape)}")
         max_slots, words = records.shape
     if history is not None:
-        _want(history, torch.uint8, "history")
+        _want_here((history, torch.uint8, "history"))
         if history.dim() != 2 or (records is not None and history.shape[0] != max_slots):
             raise KernelError("history must be [slots, n] for the slots of the records")
         max_slots, ld = history.shape
         if not begin:
             if positions is None or prefix_len is None:
                 raise KernelError("a history needs the positions that the step wrote and prefix_len")
-            _want(positions, torch.int32, "positions"); _want(prefix_len, torch.int32, "prefix_len")
+            _want_here((positions, torch.int32, "positions"), (prefix_len, torch.int32, "prefix_len"))
             if positions.numel() < groups * beams or prefix_len.numel() < groups:
                 raise KernelError("positions or prefix_len is shorter than the batch")
-    _want_here(candidates=candidates[0], stop_tokens=stop_tokens, slots=slots, scores=scores, records=records,
-               history=history, err=err)
     if groups == 0:
         return
     _check(_lib().tk_beam_advance(candidates[0].data_ptr(), candidates[1].data_ptr(), candidates[2].data_ptr(), _ptr(stop_tokens),
@@ -366,34 +366,31 @@ def reorder_slots(records, slots: torch.Tensor, parents: torch.Tensor, err: torc
     ``slots`` and ``parents`` are int32 ``[groups, seats]``; a slot belongs to one seat of one group.  A seat whose parent
     is itself is not touched, whatever else is in the tensors is left as it is.  A parent outside the group or a slot outside
     the tensors is reported through ``err`` and that seat stays as it is."""
-    _want(slots, torch.int32, "slots"); _want(parents, torch.int32, "parents"); _want(err, torch.int32, "err")
+    _want_here((slots, torch.int32, "slots"), (parents, torch.int32, "parents"), (err, torch.int32, "err"))
     if slots.dim() != 2 or parents.shape != slots.shape:
         raise KernelError(f"slots and parents must be [groups, seats], got {tuple(slots.shape)} and {tuple(parents.shape)}")
     groups, seats = slots.shape
     if not 1 <= seats <= BEAM_SEAT_LIMIT or groups > 65535:
         raise KernelError(f"records move between 1 to {BEAM_SEAT_LIMIT} seats of up to 65535 groups, got {seats} of {groups}")
-    bases, sizes, keys, max_slots = [], [], [], None
+    words, max_slots = array("q"), 0
     here = _raw_device()
     for t in records:
-        if not t.is_cuda or not t.is_contiguous() or t.dim() < 2:
+        shape = t.shape
+        if not t.is_cuda or len(shape) < 2 or not t.is_contiguous():
             raise KernelError("records must be contiguous CUDA tensors [keys, slots, ...]")
-        if max_slots is None:
-            max_slots = t.shape[1]
-        if t.shape[1] != max_slots or max_slots < 1:
+        max_slots = max_slots or shape[1]
+        if shape[1] != max_slots or max_slots < 1:
             raise KernelError("all records must have the same number of slots")
         if t.get_device() != here:
             raise KernelError(f"records must be on the current CUDA device {here}")
-        n = t.numel() * t.element_size()
-        if n:
-            bases.append(t.data_ptr()); keys.append(t.shape[0]); sizes.append(n // (t.shape[0] * max_slots))
-    _want_here(slots=slots, parents=parents, err=err)
+        if t.nbytes:
+            words.extend((t.data_ptr(), t.nbytes // (shape[0] * max_slots), shape[0]))
     if groups == 0:
         return
-    for i in range(0, len(bases), _REORDER_TENSORS):
-        n = min(_REORDER_TENSORS, len(bases) - i)
-        _check(_lib().tk_reorder_slots((ctypes.c_void_p * n)(*bases[i:i + n]), (ctypes.c_longlong * n)(*sizes[i:i + n]),
-                                       (ctypes.c_int * n)(*keys[i:i + n]), n, slots.data_ptr(), parents.data_ptr(),
-                                       err.data_ptr(), groups, seats, max_slots, _stream()), "reorder_slots")
+    for i in range(0, len(words), 3 * _REORDER_TENSORS):
+        part = words[i:i + 3 * _REORDER_TENSORS]
+        _check(_lib().tk_reorder_slots(part.buffer_info()[0], len(part) // 3, slots.data_ptr(), parents.data_ptr(), err.data_ptr(),
+                                       groups, seats, max_slots, _stream()), "reorder_slots")
 
 
 def wait_probe(limit: int, err: torch.Tensor) -> None:
@@ -1992,17 +1989,32 @@ def shared_tc_takes(n_q_heads: int, n_kv_heads: int, head_dim: int, v_dim: int, 
     return bool(library().tk_attention_shared_tc_takes(n_q_heads, n_kv_heads, head_dim, v_dim, page_size))
 
 
-def shared_splits(sms: int, groups: int, rows: int, n_q_heads: int, n_kv_heads: int, shared: SharedPrefix,
-                  window: int | None, tensor_cores: bool) -> tuple[int, int]:
-    """Parts that the shared and the other positions are cut into: enough small blocks for two an SM, none with less than 32
-    keys.  The tensor-core kernel deals its work out itself; what counts for it is whether anything is shared."""
-    keys = min(shared.max_prefix, window or shared.max_prefix)
-    if tensor_cores:
-        return int(keys > 0), 1
-    own = min(shared.max_own, window or shared.max_own)
-    blocks = groups * n_kv_heads * -(-shared.max_members * (n_q_heads // n_kv_heads) // 32)
-    n_shared = max(1, min(2 * sms // max(1, blocks), -(-keys // 32))) if keys > 0 else 0
+def shared_splits(sms: int, groups: int, rows: int, n_q_heads: int, n_kv_heads: int, members: int, prefix: int, own: int,
+                  window: int) -> tuple[int, int]:
+    """Parts that the general kernel cuts the shared and the other positions into: enough small blocks for two an SM, none with
+    less than 32 keys."""
+    if window:
+        prefix, own = min(prefix, window), min(own, window)
+    blocks = groups * n_kv_heads * -(-members * (n_q_heads // n_kv_heads) // 32)
+    n_shared = max(1, min(2 * sms // max(1, blocks), -(-prefix // 32))) if prefix > 0 else 0
     return n_shared, max(1, min(2 * sms // max(1, rows * n_kv_heads), -(-own // 32)))
+
+
+@lru_cache(maxsize=1024)
+def _shared_plan(sms: int, sizes: tuple, num_pages: int, max_prefix: int, max_own: int, window: int, has_history: bool, at: int,
+                 out_at: int, dtype: int) -> tuple[int, int, int]:
+    """Parts of the shared and the other positions, and the floats of scratch, of a call of these sizes; ``at`` and ``out_at``: where
+    its tensors begin within 16 bytes.  The tensor-core kernel deals its work out itself; what counts for it is whether
+    anything is shared."""
+    rows, groups, members, hq, hkv, d, dv, page_size = sizes
+    if dtype == 1 and shared_tc_takes(hq, hkv, d, dv, page_size):
+        n_shared, n_own = int(max_prefix > 0), 1
+    else:
+        n_shared, n_own = shared_splits(sms, groups, rows, hq, hkv, members, max_prefix, max_own, window)
+    need = library().tk_attention_shared_scratch(at, out_at, at, at, int(has_history) or None, *sizes, num_pages, n_shared, n_own, dtype)
+    if need < 0:
+        raise KernelError(f"the shared-prefix attention does not take {rows} rows of {hq} heads in {n_shared} + {n_own} parts")
+    return n_shared, n_own, need
 
 
 def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, shared: SharedPrefix,
@@ -2016,12 +2028,11 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     ``[pages, Hkv, page, d]`` (values ``dv``) and ``block_table`` ``[slots, pages]`` as in the other attention kernels, float32
     or bfloat16; ``softcap`` and ``sinks`` as in :func:`attention_plain`.  Cached keys and values must be finite wherever
     a member of the group sees them."""
-    _want(q, None, "q"); _want(out, q.dtype, "out"); _want(k_cache, q.dtype, "k_cache"); _want(v_cache, q.dtype, "v_cache")
-    dtype = dtype_code(q.dtype)
-    _want(positions, torch.int32, "positions"); _want(req_slot, torch.int32, "req_slot")
-    _want(block_table, torch.int32, "block_table"); _want(err, torch.int32, "err")
-    for name in ("group_start", "prefix_slot", "prefix_len"):
-        _want(getattr(shared, name), torch.int32, name)
+    kind, i32 = q.dtype, torch.int32
+    dtype = dtype_code(kind)
+    _want_here((q, kind, "q"), (out, kind, "out"), (k_cache, kind, "k_cache"), (v_cache, kind, "v_cache"), (positions, i32, "positions"),
+               (req_slot, i32, "req_slot"), (block_table, i32, "block_table"), (err, i32, "err"),
+               (shared.group_start, i32, "group_start"), (shared.prefix_slot, i32, "prefix_slot"), (shared.prefix_len, i32, "prefix_len"))
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4 or block_table.dim() != 2:
         raise KernelError("q must be [rows, Hq, d], the caches [pages, Hkv, page, d], the block table [slots, pages]")
     rows, hq, d = q.shape
@@ -2044,31 +2055,26 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
         raise KernelError(f"a window of {window} positions is none")
     history, ld = shared.history, 0
     if history is not None:
-        _want(history, torch.uint8, "history")
+        _want_here((history, torch.uint8, "history"))
         if history.dim() != 2 or history.shape[0] != block_table.shape[0]:
             raise KernelError("history must be [slots, n] for the slots of the block table")
         if shared.max_members > 256:
             raise KernelError(f"a history names up to 256 members of a group, got {shared.max_members}")
         ld = history.shape[1]
-    _want_sinks(sinks, hq)
-    _want_here(q=q, out=out, k_cache=k_cache, v_cache=v_cache, positions=positions, req_slot=req_slot, block_table=block_table,
-               err=err, group_start=shared.group_start, prefix_slot=shared.prefix_slot, prefix_len=shared.prefix_len,
-               history=history, sinks=sinks)
+    if sinks is not None:
+        _want_here((sinks, torch.float32, "sinks"))
+        _want_sinks(sinks, hq)
     if rows == 0:
         return
-    tensor_cores = dtype == 1 and shared_tc_takes(hq, hkv, d, dv, page_size)
-    n_shared, n_own = shared_splits(sm_count(q.device), groups, rows, hq, hkv, shared, window, tensor_cores)
-    lib = _lib()
-    sizes = (rows, groups, shared.max_members, hq, hkv, d, dv, page_size)
     ptrs = (q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr())
-    need = lib.tk_attention_shared_scratch(*ptrs, _ptr(history), *sizes, num_pages, n_shared, n_own, dtype)
-    if need < 0:
-        raise KernelError(f"the shared-prefix attention does not take {rows} rows of {hq} heads in {n_shared} + {n_own} parts")
+    sizes = (rows, groups, shared.max_members, hq, hkv, d, dv, page_size)
+    n_shared, n_own, need = _shared_plan(sm_count(q.device), sizes, num_pages, shared.max_prefix, shared.max_own, window or 0,
+                                         history is not None, (ptrs[0] | ptrs[2] | ptrs[3]) & 15, ptrs[1] & 15, dtype)
     scratch = torch.empty(need, dtype=torch.float32, device=q.device)
-    _check(lib.tk_attention_shared(*ptrs, shared.group_start.data_ptr(), shared.prefix_slot.data_ptr(), shared.prefix_len.data_ptr(),
-                                   positions.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), _ptr(history), _ptr(sinks),
-                                   scratch.data_ptr(), err.data_ptr(), *sizes, block_table.shape[1], num_pages, block_table.shape[0], ld,
-                                   int(window or 0), n_shared, n_own, float(scale), float(softcap or 0.0), dtype, _stream()),
+    _check(_lib().tk_attention_shared(*ptrs, shared.group_start.data_ptr(), shared.prefix_slot.data_ptr(), shared.prefix_len.data_ptr(),
+                                      positions.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), _ptr(history), _ptr(sinks),
+                                      scratch.data_ptr(), err.data_ptr(), *sizes, block_table.shape[1], num_pages, block_table.shape[0],
+                                      ld, window or 0, n_shared, n_own, scale, softcap or 0.0, dtype, _stream()),
            "attention_shared")
 
 
