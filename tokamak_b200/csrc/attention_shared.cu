@@ -307,7 +307,7 @@ TK_API int tk_attention_shared_tc_takes(int n_q_heads, int n_kv_heads, int head_
   return tk::shared_tc_takes(p);
 }
 
-// scratch: 16-byte aligned, as many floats as tk_attention_shared_scratch says for the same arguments.
+// scratch: 32-byte aligned, as many floats as tk_attention_shared_scratch says for the same arguments.
 static int shared_params(tk::SharedParams& p, const void* q, void* out, const void* k_cache, const void* v_cache, int n_rows, int n_groups,
                          int max_members, int n_q_heads, int n_kv_heads, int head_dim, int v_dim, int page_size, int num_pages, int n_shared,
                          int n_own, const unsigned char* history, int dtype) {
@@ -351,7 +351,7 @@ TK_API int tk_attention_shared(const void* q, void* out, const void* k_cache, co
   const int bad = shared_params(p, q, out, k_cache, v_cache, n_rows, n_groups, max_members, n_q_heads, n_kv_heads, head_dim, v_dim, page_size,
                                 num_pages, n_shared, n_own, history, dtype);
   if (bad != 0) return bad;
-  if (max_slots < 1 || max_pages < 1 || (history != nullptr && history_ld < 1) || ((uintptr_t)scratch & 15) != 0) return (int)cudaErrorInvalidValue;
+  if (max_slots < 1 || max_pages < 1 || (history != nullptr && history_ld < 1) || ((uintptr_t)scratch & 31) != 0) return (int)cudaErrorInvalidValue;
   p.group_start = group_start; p.prefix_slot = prefix_slot; p.prefix_len = prefix_len; p.positions = positions; p.req_slot = req_slot;
   p.block_table = block_table; p.sinks = sinks; p.err = err; p.scratch = scratch;
   p.max_pages = max_pages; p.max_slots = max_slots; p.history_ld = history_ld; p.window = window;

@@ -200,6 +200,11 @@ struct Segment {          // what a block does of one triple
   int group_row0, prefix;
 };
 
+__device__ __forceinline__ void st_global_32(float* dst, const uint32_t* r) {          // 32 bytes, on 32
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n"
+               ::"l"(dst), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+
 __device__ __forceinline__ float sp_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -242,11 +247,15 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = p.n_q_heads / p.n_kv_heads, mpt = s.members_per_tile;
+  if (threadIdx.x >= 32 && threadIdx.x < 35) {
+    const CUtensorMap* m = threadIdx.x == 32 ? &map_k : threadIdx.x == 33 ? &map_v : &map_q;
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"(m) : "memory");
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSpStages; ++i) {
-      mbar_init(gt_smem_u32(&k_full[i]), 1);
+      mbar_init(gt_smem_u32(&k_full[i]), 32);       // the lanes of its loads' warp, and what TMA brings
       mbar_init(gt_smem_u32(&k_empty[i]), 2);       // both issuers
-      mbar_init(gt_smem_u32(&v_full[i]), 1);
+      mbar_init(gt_smem_u32(&v_full[i]), 32);
       mbar_init(gt_smem_u32(&v_empty[i]), 2);       // both issuers
     }
     for (int t = 0; t < 2; ++t) {
@@ -343,15 +352,6 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       const int ppt = kSpBN / kpl;                                   // loads of a tile (times SUB halves): at most 8
       const bool loader = lane < ppt * SUB;
       const int c = lane % SUB, u = lane / SUB;
-      uint32_t tail = 0;                                             // barrier of a tile whose cp.asyncs have not been announced
-      auto announce = [&](bool all) {
-        if (tail == 0) return;
-        if (all) cp_async_wait<0>(); else cp_async_wait<1>();
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(tail);
-        tail = 0;
-      };
       for (int i = 0; i < n_seg && ok; ++i, ++n_seg_done) {
         const Segment x = s_seg[i];
         const int n_prefix = min(x.n_tiles, max(0, x.prefix_tiles - x.tile0));       // tiles of the prefix come first
@@ -409,8 +409,10 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
               rows_next = batch_of(batch_now + 1);
             }
             const int row = __shfl_sync(0xffffffffu, rows_now, w & 31);
-            announce(true);
-            if (lane == 0) mbar_expect_tx(bar, KV_BYTES);
+            if (lane == 0) {
+              mbar_expect_tx(bar, KV_BYTES);
+              asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 31;\n" ::"r"(bar) : "memory");
+            }
             __syncwarp();
             if (loader) tma_load_2d(dst0 + c * KSUB_BYTES + u * kpl * 128, map, c * 64, row, bar);
           } else {
@@ -424,14 +426,12 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
               cp_async16(dst0 + (ch / 8) * KSUB_BYTES + r * 128 + (((ch % 8) ^ (r & 7)) * 16), cache + (size_t)(from < 0 ? 0 : from) * D + ch * 8,
                          from >= 0);
             }
-            cp_async_commit();
-            announce(false);                                         // the tile before, now that this one is on its way
-            tail = bar;
+            // a lane arrives when its copies have: nobody waits for them here
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
           }
           if (++st == kSpStages) { st = 0; ph ^= 1u; }
           if (!values && j == min(1, x.n_tiles - 1)) {
             // the queries, behind the first keys
-            announce(true);                                          // the segment before may be waiting for it
             if (n_seg_done > 0) {
               ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (n_seg_done - 1u) & 1u, abort_flag));
               if (!ok) { if (lane == 0) { set_error(p.err, kErrWait, 46, i, 0); *abort_flag = 1; } break; }
@@ -450,7 +450,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           }
         }
       }
-      announce(true);
+      cp_async_wait<0>();
     } else if (warp == 1 || warp == kSpSecondIssuer) {
       // ---- products of softmax group t --------------------------------------------------------------------------------------
       // The whole warp walks and waits; one thread issues.  Both issuers give every stage back; one that is not theirs once they
@@ -476,7 +476,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         if (++st_v == kSpStages) { st_v = 0; ph_v ^= 1u; }
       };
       for (int i = 0; i < n_seg && ok; ++i, ++n_seg_done) {
-        const int n_tiles = s_seg[i].n_tiles;
+        const int n_tiles = s_seg[i].n_tiles, n_prefix = s_seg[i].prefix_tiles - s_seg[i].tile0;
         const bool both = s_seg[i].members > mpt;          // two tiles of rows; otherwise the groups take turns at the key tiles
         const int n_mine = both ? n_tiles : (n_tiles + 1 - t) / 2;
         if (!wait(q_full, n_seg_done & 1u, 4)) break;
@@ -487,6 +487,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           if (n < n_mine) {
             if (!both && (t == 1 || n > 0)) pass_keys();
             if (!wait(gt_smem_u32(&k_full[st]), ph, 1)) break;
+            if ((both ? n : 2 * n + t) >= n_prefix) fence_async_shared();          // rows that cp.async brought
             tc_fence_after();
             const int bf = (int)((units0 + (uint32_t)n) & 1u);
             if (elect_one()) {
@@ -510,6 +511,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             if (!wait(gt_smem_u32(&v_full[st_v]), ph_v, 2)) break;
             if (!wait(p_full(t, bf), (mine >> 1) & 1u, 3)) break;
             if (n == 1 && outs0 > 0 && !wait(o_empty(t), (outs0 - 1u) & 1u, 5)) break;          // the segment before has been read
+            if ((both ? n - 1 : 2 * n - 2 + t) >= n_prefix) fence_async_shared();
             tc_fence_after();
             if (elect_one()) {
               const uint64_t db0 = desc_v + (uint64_t)(st_v * (KV_BYTES >> 4));
@@ -679,9 +681,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
               tmem_wait_ld();
               if (row < n_rows && l_sum > 0.0f) {
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                  reinterpret_cast<uint4*>(po + c * 32)[q] = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
-                }
+                for (int q = 0; q < 4; ++q) st_global_32(po + c * 32 + 8 * q, &o[8 * q]);          // (16 bytes at a time: twice the time)
               }
             }
             tc_fence_before();
@@ -1055,7 +1055,7 @@ static bool has_shared(const SharedParams& p) { return p.n_shared > 0 || p.histo
 static SharedPlan layout(const SharedParams& p, int sms, long long* floats) {
   SharedPlan s = {};
   long long at = 0;
-  auto take = [&](long long n) { float* q = p.scratch + at; at += (n + 3) / 4 * 4; return q; };
+  auto take = [&](long long n) { float* q = p.scratch + at; at += (n + 7) / 8 * 8; return q; };
   const long long pairs = (long long)p.n_rows * p.n_q_heads;
   if (has_shared(p)) {
     s.ints = reinterpret_cast<int*>(take(kPlanHead + (long long)p.n_groups * kPlanRecord));
