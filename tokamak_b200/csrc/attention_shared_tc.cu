@@ -615,7 +615,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             if (capped) {
 #pragma unroll
               for (int c = 0; c < kSpBN; ++c) {
-                if (sv[c] != -INFINITY) sv[c] = capped_score_log2(sv[c], p.scale_log2, p.cap_log2, p.inv_cap);
+                // (a branch around it, to skip what is masked, would let no two of them overlap: 160 clocks an element)
+                const float y = capped_score_log2(sv[c], p.scale_log2, p.cap_log2, p.inv_cap);
+                sv[c] = sv[c] == -INFINITY ? -INFINITY : y;
               }
               if (mx != -INFINITY) mx = capped_score_log2(mx, p.scale_log2, p.cap_log2, p.inv_cap);
             }
