@@ -25,6 +25,7 @@ namespace tk {
 constexpr int kSelThreads = 256;
 constexpr int kSelEach = 16;                                   // logits of a thread in one tile
 constexpr int kSelTile = kSelThreads * kSelEach;               // logits of a tile
+constexpr int kSelCheck = 3;                                   // tiles between two looks at how many were set aside
 constexpr int kSelKept = 512;                                  // elements set aside that are left when they are thinned out
 constexpr int kSelBuffer = 2048;                               // elements set aside
 constexpr int kJoinThreads = 512;                              // and so many are ranked by comparing each with each
@@ -102,6 +103,26 @@ __device__ __forceinline__ U block_threshold_of(int k, int most, bool any, U val
   return t;
 }
 
+// Those of the n elements set aside that are at or above t are kept.  Returns how many.
+__device__ __noinline__ int keep_from(unsigned long long* buf, int* s_count, int n, unsigned long long t) {
+  constexpr int PER = kSelBuffer / kSelThreads;
+  unsigned long long mine[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = i * kSelThreads + threadIdx.x;
+    mine[i] = at < n ? buf[at] : 0ull;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) *s_count = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (mine[i] != 0ull && mine[i] >= t) buf[atomicAdd(s_count, 1)] = mine[i];
+  }
+  __syncthreads();
+  return *s_count;
+}
+
 // Of the n elements set aside those of tokens before `limit` are kept, and of these, where they are more than kSelKept, the k
 // largest (and a few behind them, up to kSelKept).  Returns how many.  (Elements are distinct.)
 __device__ __noinline__ int thin_out(unsigned long long* buf, int* s_count, int n, int k, unsigned int limit) {
@@ -168,7 +189,11 @@ __device__ __forceinline__ float2 terms_f32(float x, float y, float ref) {
   return d;
 }
 
-__global__ void __launch_bounds__(kSelThreads, 4)
+// kPerSm: blocks on an SM at a time.  Four leave a thread 64 registers, and it keeps some of its values in memory; where there are
+// no more blocks than three an SM take (8 groups of 4 beams over 151,936 tokens: 416), they are faster by themselves: 15.3 us
+// against 17.0 for the selection.  512 rows of 100,003 logits, more than that: 68 us with three, 55 with four.
+template <int kPerSm>
+__global__ void __launch_bounds__(kSelThreads, kPerSm)
 beam_segments_kernel(SelectParams p) {
   pdl_trigger();
   __shared__ unsigned long long s_buf[kSelBuffer];
@@ -238,17 +263,16 @@ beam_segments_kernel(SelectParams p) {
   float least = o_least <= ordered_f32(-INFINITY) ? -INFINITY : from_ordered_f32(o_least);
   double sum = 0.0;
 
-  // More elements than the buffer holds: those of the tile are set aside again, a row of a block's threads at a time, with the
-  // threshold raised in between.  (Logits in rising order, or many equal ones.)
-  auto crowded = [&](int t0, const float (&e)[kSelEach], bool first) {
-    __syncthreads();
+  // More elements than the buffer holds: those of the tiles from t0 to t1, before which all were held, are set aside again, a row
+  // of a block's threads at a time, with the threshold raised in between.  (Logits in rising order, or many equal ones.)
+  auto crowded = [&](int t0, int t1, bool first) {
     int n = thin_out(s_buf, &s_count, min(s_count, kSelBuffer), p.k, (unsigned int)t0);
     bool reached = first;                         // whether an element equal to the threshold still counts
     if (n >= p.k) { least = lowest_of(s_buf, n); reached = false; }
-#pragma unroll
-    for (int j = 0; j < kSelEach; ++j) {
-      const int i = t0 + j * kSelThreads + (int)threadIdx.x;
-      if (i < end && (reached ? e[j] >= least : e[j] > least)) set_aside(i, e[j]);
+    for (int i0 = t0; i0 < min(t1, end); i0 += kSelThreads) {
+      const int i = i0 + (int)threadIdx.x;
+      const float v = i < end ? x[i] : -INFINITY;
+      if (i < end && (reached ? fmaxf(v, -INFINITY) >= least : v > least)) set_aside(i, fmaxf(v, -INFINITY));
       __syncthreads();
       n = s_count;
       __syncthreads();
@@ -263,7 +287,7 @@ beam_segments_kernel(SelectParams p) {
   for (int j = 0; j < kSelEach; ++j) {
     if (cur[j] >= least && begin + j * kSelThreads + (int)threadIdx.x < end) set_aside(begin + j * kSelThreads + (int)threadIdx.x, cur[j]);
   }
-  if (__syncthreads_or(s_count > kSelBuffer)) crowded(begin, cur, true);
+  if (__syncthreads_or(s_count > kSelBuffer)) crowded(begin, begin + kSelTile, true);
 
   // The sum of a tile's exponentials.  The reference is the first tile's maximum; it is raised (and what has been
   // summed so far scaled down) only where an exponent would leave the range that the sums hold.
@@ -287,6 +311,9 @@ beam_segments_kernel(SelectParams p) {
     }
   };
   add_tile(cur, top);
+  float best = top;                               // of the thread, so far
+  int check_at = begin + (1 + kSelCheck) * kSelTile;          // where the buffer is looked at next
+  int raise_at = begin + 4 * kSelTile;            // and when it raises the threshold next
   for (int t0 = begin + kSelTile; t0 < end; t0 += kSelTile) {
 #pragma unroll
     for (int j = 0; j < kSelEach; ++j) cur[j] = nxt[j];
@@ -294,13 +321,30 @@ beam_segments_kernel(SelectParams p) {
     clean(cur);
     const float m = tile_max(cur);
     if (m > least) {                              // -inf behind the segment's end is never more
+      unsigned int bits = 0u;
 #pragma unroll
-      for (int j = 0; j < kSelEach; ++j) {
-        if (cur[j] > least) set_aside(t0 + j * kSelThreads + (int)threadIdx.x, cur[j]);
+      for (int j = 0; j < kSelEach; ++j) bits |= cur[j] > least ? 1u << j : 0u;
+      if ((bits & (bits - 1u)) == 0u) {
+        set_aside(t0 + (__ffs(bits) - 1) * kSelThreads + (int)threadIdx.x, m);
+      } else {
+        for (; bits != 0u; bits &= bits - 1u) {   // read again: a register cannot be picked at run time
+          const int i = t0 + (__ffs(bits) - 1) * kSelThreads + (int)threadIdx.x;
+          set_aside(i, x[i]);
+        }
       }
     }
     add_tile(cur, m);
-    if (__syncthreads_or(s_count > kSelBuffer)) crowded(t0, cur, false);
+    best = fmaxf(best, m);
+    if (t0 + kSelTile < check_at && t0 + kSelTile < end) continue;
+    if (__syncthreads_or(s_count > kSelBuffer)) crowded(check_at - kSelCheck * kSelTile, t0 + kSelTile, false);
+    check_at += kSelCheck * kSelTile;
+    // The threshold that the first tile gave lets one logit in kSelTile / K pass, and whatever passes costs its whole warp.  Once
+    // four times as many have been seen, K of the threads' best so far are at or above a higher one.
+    if (t0 + kSelTile >= raise_at && end - t0 > 4 * kSelTile) {
+      raise_at += 3 * (raise_at - begin);
+      const unsigned int o = block_threshold_of<unsigned int>(p.k, p.k + p.k / 2, begin + (int)threadIdx.x < end, ordered_f32(best));
+      if (o > ordered_f32(-INFINITY)) least = fmaxf(least, from_ordered_f32(o));
+    }
   }
   __syncthreads();
 
@@ -311,6 +355,10 @@ beam_segments_kernel(SelectParams p) {
   }
   int n = s_count;
   __syncthreads();
+  if (n > 2 * p.k && n > 64) {                    // ranking them all would compare each with each
+    const unsigned int o = block_threshold_of<unsigned int>(p.k, p.k + p.k / 2, begin + (int)threadIdx.x < end, ordered_f32(best));
+    n = keep_from(s_buf, &s_count, n, (unsigned long long)o << 32);
+  }
   if (n > kSelKept) n = thin_out(s_buf, &s_count, n, p.k, 0xffffffffu);
   float ref_all = -INFINITY;
 #pragma unroll
@@ -366,6 +414,9 @@ beam_join_kernel(SelectParams p) {
   if (threadIdx.x == 0) s_count = 0;
   s_rank[threadIdx.x] = 0;
   pdl_wait();
+  const unsigned long long* elems = p.seg_key + row0 * per_row;
+  const bool one_each = n <= kJoinThreads;                     // a thread has one element: it stays in a register
+  const unsigned long long my_elem = one_each && (int)threadIdx.x < n ? __ldcg(elems + threadIdx.x) : 0ull;
   for (int b = warp; b < p.beams; b += kJoinThreads / 32) {
     const double2* seg = reinterpret_cast<const double2*>(p.seg_sum) + (row0 + b) * p.segments;
     const double2 first = lane < p.segments ? __ldcg(seg + lane) : make_double2(-INFINITY, 0.0);
@@ -392,7 +443,6 @@ beam_join_kernel(SelectParams p) {
     if (!(key > -INFINITY)) key = -INFINITY;                   // dead beams, -inf logits, rows of -inf alone
     return ordered_f64(key);
   };
-  const unsigned long long* elems = p.seg_key + row0 * per_row;
   auto any_key = [&](int i) {
     const unsigned long long elem = __ldcg(elems + i);
     return elem == 0ull ? 0ull : key_of(i / per_row, elem);
@@ -400,97 +450,102 @@ beam_join_kernel(SelectParams p) {
   // Keys as floats, rounded down, are in the keys' order but for what they round away, and half the bits to look at.
   auto as_float = [&](unsigned long long key) { return key == 0ull ? 0u : ordered_f32(__double2float_rd(from_ordered_f64(key))); };
   auto from_float = [&](unsigned int t32) { return t32 <= ordered_f32(-INFINITY) ? 1ull : ordered_f64((double)from_ordered_f32(t32)); };
-  unsigned long long t = 1ull;                                   // everything there is
-  if (lists > p.k) {
-    for (int i = threadIdx.x; i < lists; i += kJoinThreads) s_key[i * p.k] = any_key(i * p.k);
-    __syncthreads();
-    if (lists <= kJoinThreads) {
-      const unsigned long long key = (int)threadIdx.x < lists ? s_key[threadIdx.x * p.k] : 0ull;
-      t = from_float(block_threshold_of<unsigned int>(p.k, p.k, key != 0ull, as_float(key)));
-    } else {
-      t = from_float(block_threshold<kJoinThreads, unsigned int>(p.k, p.k + p.k / 4, [&](unsigned int trial) {
-        int c = 0;
-        for (int i = threadIdx.x; i < lists; i += kJoinThreads) c += as_float(s_key[i * p.k]) >= trial ? 1 : 0;
-        return c;
-      }));
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kJoinThreads) {
-      const int list = i / p.k, first = list * p.k;
-      if (i != first) s_key[i] = s_key[first] >= t ? any_key(i) : 0ull;
-    }
-  } else {
-    for (int i = threadIdx.x; i < n; i += kJoinThreads) s_key[i] = any_key(i);
-  }
-  __syncthreads();
   // what comes after the key: the logit where it decides, then the place
-  auto second_of = [&](int i) {
-    const unsigned long long elem = __ldcg(elems + i);
+  auto second_of = [&](int i, unsigned long long key, unsigned long long elem) {
     const unsigned int place = (unsigned int)(i / per_row) * (unsigned int)p.vocab + (0xffffffffu - (unsigned int)elem);
-    const unsigned int logit = s_key[i] == ordered_f64(-INFINITY) ? 0u : (unsigned int)(elem >> 32);
+    const unsigned int logit = key == ordered_f64(-INFINITY) ? 0u : (unsigned int)(elem >> 32);
     return ((unsigned long long)logit << 32) | (0xffffffffu - place);
   };
-  auto gather = [&](unsigned long long t, unsigned long long t2) {
-    __syncthreads();
-    if (threadIdx.x == 0) s_count = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kJoinThreads) {
-      const unsigned long long key = s_key[i];
-      if (key < t) continue;
-      const unsigned long long second = second_of(i);
-      if (key > t || second >= t2) {
-        const int at = atomicAdd(&s_count, 1);
-        if (at < kJoinThreads) { s_best[at] = key; s_second[at] = second; }
+  const unsigned long long my_key = my_elem == 0ull ? 0ull : key_of((int)threadIdx.x / per_row, my_elem);
+  int m = 0;
+  if (!one_each) {
+    unsigned long long t = 1ull;                                   // everything there is
+    if (lists > p.k) {
+      for (int i = threadIdx.x; i < lists; i += kJoinThreads) s_key[i * p.k] = any_key(i * p.k);
+      __syncthreads();
+      if (lists <= kJoinThreads) {
+        const unsigned long long key = (int)threadIdx.x < lists ? s_key[threadIdx.x * p.k] : 0ull;
+        t = from_float(block_threshold_of<unsigned int>(p.k, p.k, key != 0ull, as_float(key)));
+      } else {
+        t = from_float(block_threshold<kJoinThreads, unsigned int>(p.k, p.k + p.k / 4, [&](unsigned int trial) {
+          int c = 0;
+          for (int i = threadIdx.x; i < lists; i += kJoinThreads) c += as_float(s_key[i * p.k]) >= trial ? 1 : 0;
+          return c;
+        }));
       }
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += kJoinThreads) {
+        const int list = i / p.k, first = list * p.k;
+        if (i != first) s_key[i] = s_key[first] >= t ? any_key(i) : 0ull;
+      }
+    } else {
+      for (int i = threadIdx.x; i < n; i += kJoinThreads) s_key[i] = any_key(i);
     }
     __syncthreads();
-    return s_count;
-  };
-  int m = gather(t, 0ull);
-  if (m > kJoinThreads) {
-    // more than can be ranked: a threshold over all of them
-    t = max(t, from_float(block_threshold<kJoinThreads, unsigned int>(p.k, kJoinThreads, [&](unsigned int trial) {
-      int c = 0;
-      for (int i = threadIdx.x; i < n; i += kJoinThreads) c += as_float(s_key[i]) >= trial ? 1 : 0;
-      return c;
-    })));
-    m = gather(t, 0ull);
-  }
-  if (m > kJoinThreads) {
-    // Where more than can be ranked share the K-th key (beams that all are dead, rows of equal logits), the same search goes on
-    // over all bits of the keys, and then over what comes after the key.
-    auto at_least = [&](unsigned long long trial) {
-      int c = 0;
-      for (int i = threadIdx.x; i < n; i += kJoinThreads) c += s_key[i] >= trial ? 1 : 0;
-      return c;
+    auto gather = [&](unsigned long long t, unsigned long long t2) {
+      __syncthreads();
+      if (threadIdx.x == 0) s_count = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += kJoinThreads) {
+        const unsigned long long key = s_key[i];
+        if (key < t) continue;
+        const unsigned long long second = second_of(i, s_key[i], __ldcg(elems + i));
+        if (key > t || second >= t2) {
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kJoinThreads) { s_best[at] = key; s_second[at] = second; }
+        }
+      }
+      __syncthreads();
+      return s_count;
     };
-    t = max(1ull, block_threshold<kJoinThreads, unsigned long long>(p.k, kJoinThreads, at_least));
-    unsigned long long t2 = 0ull;
-    __shared__ int s_above;
-    if (threadIdx.x == 0) s_above = 0;
-    __syncthreads();
-    const int above_here = at_least(t + 1ull);
-    if (above_here > 0) atomicAdd(&s_above, above_here);
-    __syncthreads();
-    const int above = s_above;
-    if (above < p.k) {
-      t2 = block_threshold<kJoinThreads, unsigned long long>(p.k - above, kJoinThreads - above, [&](unsigned long long trial) {
+    m = gather(t, 0ull);
+    if (m > kJoinThreads) {
+      // more than can be ranked: a threshold over all of them
+      t = max(t, from_float(block_threshold<kJoinThreads, unsigned int>(p.k, kJoinThreads, [&](unsigned int trial) {
         int c = 0;
-        for (int i = threadIdx.x; i < n; i += kJoinThreads) c += (s_key[i] == t && second_of(i) >= trial) ? 1 : 0;
+        for (int i = threadIdx.x; i < n; i += kJoinThreads) c += as_float(s_key[i]) >= trial ? 1 : 0;
         return c;
-      });
+      })));
+      m = gather(t, 0ull);
     }
-    m = gather(t, t2);
+    if (m > kJoinThreads) {
+      // Where more than can be ranked share the K-th key (beams that all are dead, rows of equal logits), the same search goes on
+      // over all bits of the keys, and then over what comes after the key.
+      auto at_least = [&](unsigned long long trial) {
+        int c = 0;
+        for (int i = threadIdx.x; i < n; i += kJoinThreads) c += s_key[i] >= trial ? 1 : 0;
+        return c;
+      };
+      t = max(1ull, block_threshold<kJoinThreads, unsigned long long>(p.k, kJoinThreads, at_least));
+      unsigned long long t2 = 0ull;
+      __shared__ int s_above;
+      if (threadIdx.x == 0) s_above = 0;
+      __syncthreads();
+      const int above_here = at_least(t + 1ull);
+      if (above_here > 0) atomicAdd(&s_above, above_here);
+      __syncthreads();
+      const int above = s_above;
+      if (above < p.k) {
+        t2 = block_threshold<kJoinThreads, unsigned long long>(p.k - above, kJoinThreads - above, [&](unsigned long long trial) {
+          int c = 0;
+          for (int i = threadIdx.x; i < n; i += kJoinThreads) c += (s_key[i] == t && second_of(i, s_key[i], __ldcg(elems + i)) >= trial) ? 1 : 0;
+          return c;
+        });
+      }
+      m = gather(t, t2);
+    }
   }
-  if (m > 64 && m > 2 * p.k) {
+  if (one_each || (m > 64 && m > 2 * p.k)) {
     // ranking compares each with each: a threshold over them first
     const bool there = (int)threadIdx.x < m;
-    const unsigned long long key = there ? s_best[threadIdx.x] : 0ull, second = there ? s_second[threadIdx.x] : 0ull;
-    const unsigned long long least = from_float(block_threshold_of<unsigned int>(p.k, p.k + p.k / 4, there, as_float(key)));
+    const unsigned long long key = one_each ? my_key : there ? s_best[threadIdx.x] : 0ull;
+    const unsigned long long second = one_each ? second_of(threadIdx.x, my_key, my_elem) : there ? s_second[threadIdx.x] : 0ull;
+    const bool any = key != 0ull;
+    const unsigned long long least = from_float(block_threshold_of<unsigned int>(p.k, p.k + p.k / 4, any, as_float(key)));
     __syncthreads();
     if (threadIdx.x == 0) s_count = 0;
     __syncthreads();
-    if (there && key >= least) {
+    if (any && key >= least) {
       const int at = atomicAdd(&s_count, 1);
       s_best[at] = key;
       s_second[at] = second;
@@ -735,7 +790,9 @@ TK_API int tk_beam_select(const float* logits, long long ld, const float* scores
     if (e != cudaSuccess) return (int)e;
     configured[dev] = true;
   }
-  e = tk::launch(tk::beam_segments_kernel, dim3(segments, groups * beams), dim3(tk::kSelThreads), 0, stream, p);
+  const bool few = (long long)segments * groups * beams <= 3LL * tk::device_sm_count();
+  e = tk::launch(few ? tk::beam_segments_kernel<3> : tk::beam_segments_kernel<4>, dim3(segments, groups * beams), dim3(tk::kSelThreads), 0,
+                 stream, p);
   if (e != cudaSuccess) return (int)e;
   return (int)tk::launch(tk::beam_join_kernel, dim3(groups), dim3(tk::kJoinThreads), join_smem, stream, p);
 }
