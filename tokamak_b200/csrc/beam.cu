@@ -25,7 +25,7 @@ namespace tk {
 constexpr int kSelThreads = 256;
 constexpr int kSelEach = 16;                                   // logits of a thread in one tile
 constexpr int kSelTile = kSelThreads * kSelEach;               // logits of a tile
-constexpr int kSelCheck = 3;                                   // tiles between two looks at how many were set aside
+constexpr int kSelCheck = 4;                                   // tiles between two looks at how many were set aside
 constexpr int kSelKept = 512;                                  // elements set aside that are left when they are thinned out
 constexpr int kSelBuffer = 2048;                               // elements set aside
 constexpr int kJoinThreads = 512;                              // and so many are ranked by comparing each with each
@@ -312,8 +312,6 @@ beam_segments_kernel(SelectParams p) {
   };
   add_tile(cur, top);
   float best = top;                               // of the thread, so far
-  int check_at = begin + (1 + kSelCheck) * kSelTile;          // where the buffer is looked at next
-  int raise_at = begin + 4 * kSelTile;            // and when it raises the threshold next
   for (int t0 = begin + kSelTile; t0 < end; t0 += kSelTile) {
 #pragma unroll
     for (int j = 0; j < kSelEach; ++j) cur[j] = nxt[j];
@@ -335,13 +333,14 @@ beam_segments_kernel(SelectParams p) {
     }
     add_tile(cur, m);
     best = fmaxf(best, m);
-    if (t0 + kSelTile < check_at && t0 + kSelTile < end) continue;
-    if (__syncthreads_or(s_count > kSelBuffer)) crowded(check_at - kSelCheck * kSelTile, t0 + kSelTile, false);
-    check_at += kSelCheck * kSelTile;
+    const int seen = t0 + kSelTile - begin;       // a number of tiles, but for the last
+    if (seen % (kSelCheck * kSelTile) != 0 && t0 + kSelTile < end) continue;
+    if (__syncthreads_or(s_count > kSelBuffer)) {
+      crowded(begin + max(kSelTile, (seen / kSelTile - 1) / kSelCheck * (kSelCheck * kSelTile)), t0 + kSelTile, false);
+    }
     // The threshold that the first tile gave lets one logit in kSelTile / K pass, and whatever passes costs its whole warp.  Once
-    // four times as many have been seen, K of the threads' best so far are at or above a higher one.
-    if (t0 + kSelTile >= raise_at && end - t0 > 4 * kSelTile) {
-      raise_at += 3 * (raise_at - begin);
+    // four times (or sixteen times) as many have been seen, K of the threads' best so far are at or above a higher one.
+    if ((seen == 4 * kSelTile || seen == 16 * kSelTile) && end - t0 > 4 * kSelTile) {
       const unsigned int o = block_threshold_of<unsigned int>(p.k, p.k + p.k / 2, begin + (int)threadIdx.x < end, ordered_f32(best));
       if (o > ordered_f32(-INFINITY)) least = fmaxf(least, from_ordered_f32(o));
     }
