@@ -23,7 +23,8 @@
 namespace tk {
 
 constexpr int kSelThreads = 256;
-constexpr int kSelEach = 16;                                   // logits of a thread in one tile
+constexpr int kSelEach = 14;                                   // logits of a thread in one tile (16: 60 us for 512 rows of 100,003 instead
+                                                               // of 54, more than the registers hold; 10: 58)
 constexpr int kSelTile = kSelThreads * kSelEach;               // logits of a tile
 constexpr int kSelCheck = 4;                                   // tiles between two looks at how many were set aside
 constexpr int kSelKept = 512;                                  // elements set aside that are left when they are thinned out
@@ -304,10 +305,14 @@ beam_segments_kernel(SelectParams p) {
       ref = m;
     }
 #pragma unroll
-    for (int j = 0; j < kSelEach; j += 4) {
+    for (int j = 0; j + 3 < kSelEach; j += 4) {
       const float2 a = terms_f32(e[j], e[j + 1], ref), b = terms_f32(e[j + 2], e[j + 3], ref);
       const float2 c = add2(a, b);
       sum += (double)(c.x + c.y);
+    }
+    if (kSelEach % 4 == 2) {
+      const float2 a = terms_f32(e[kSelEach - 2], e[kSelEach - 1], ref);
+      sum += (double)(a.x + a.y);
     }
   };
   add_tile(cur, top);

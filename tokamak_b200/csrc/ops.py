@@ -236,7 +236,7 @@ def _want_here(*wants) -> None:
 BEAM_MAX = 64                     # beams of a group
 BEAM_MAX_CANDIDATES = 256
 _BEAM_MAX_ENTRIES = 16384         # beams * segments * candidates that the kernel which joins a group's segments takes
-_BEAM_TILE = 4096                 # logits that a block has in flight at a time
+_BEAM_TILE = 3584                 # logits that a block has in flight at a time
 BEAM_SEAT_LIMIT = 64              # seats of a group that reorder_slots moves between
 
 
