@@ -352,9 +352,23 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       const int ppt = kSpBN / kpl;                                   // loads of a tile (times SUB halves): at most 8
       const bool loader = lane < ppt * SUB;
       const int c = lane % SUB, u = lane / SUB;
+      auto load_queries = [&](const Segment& x) {
+        const int n_q = x.members > mpt ? 2 : 1;
+        mbar_expect_tx(q_full, (uint32_t)(n_q * SUB * mpt * per * 128));
+        for (int t = 0; t < n_q; ++t) {
+#pragma unroll
+          for (int cc = 0; cc < SUB; ++cc) {
+            tma_load_3d(q_smem + t * Q_BYTES + cc * (kSpBM * 128), &map_q, cc * 64, x.hkv * per, x.row0 + t * mpt, q_full);
+          }
+        }
+      };
       for (int i = 0; i < n_seg && ok; ++i, ++n_seg_done) {
         const Segment x = s_seg[i];
         const int n_prefix = min(x.n_tiles, max(0, x.prefix_tiles - x.tile0));       // tiles of the prefix come first
+        if (values && n_seg_done == 0) {                             // a block's first queries, while the other warp loads keys
+          if (lane == 0) load_queries(x);
+          __syncwarp();
+        }
         // ---- pages of the prefix's tiles: lane l of a batch has load number 32 * batch + l of the segment ----
         const int* table = p.block_table + (size_t)x.slot * p.max_pages;
         auto batch_of = [&](int batch) {
@@ -430,22 +444,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(bar) : "memory");
           }
           if (++st == kSpStages) { st = 0; ph ^= 1u; }
-          if (!values && j == min(1, x.n_tiles - 1)) {
-            // the queries, behind the first keys
-            if (n_seg_done > 0) {
-              ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (n_seg_done - 1u) & 1u, abort_flag));
-              if (!ok) { if (lane == 0) { set_error(p.err, kErrWait, 46, i, 0); *abort_flag = 1; } break; }
-            }
-            if (lane == 0) {
-              const int n_q = x.members > mpt ? 2 : 1;
-              mbar_expect_tx(q_full, (uint32_t)(n_q * SUB * mpt * per * 128));
-              for (int t = 0; t < n_q; ++t) {
-#pragma unroll
-                for (int cc = 0; cc < SUB; ++cc) {
-                  tma_load_3d(q_smem + t * Q_BYTES + cc * (kSpBM * 128), &map_q, cc * 64, x.hkv * per, x.row0 + t * mpt, q_full);
-                }
-              }
-            }
+          if (!values && n_seg_done > 0 && j == min(1, x.n_tiles - 1)) {
+            // the queries, behind the first keys, once those of the segment before are done with
+            ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (n_seg_done - 1u) & 1u, abort_flag));
+            if (!ok) { if (lane == 0) { set_error(p.err, kErrWait, 46, i, 0); *abort_flag = 1; } break; }
+            if (lane == 0) load_queries(x);
             __syncwarp();
           }
         }
@@ -823,13 +826,17 @@ constexpr int kSoTile = 16;           // keys of a warp's tile
 constexpr int kSoChunk = 1024;        // keys whose places are looked up at a time
 
 template <int D, int STAGES>
-constexpr int own_smem() {
-  return kSoWarps * STAGES * 2 * kSoTile * D * 2 > kSoWarps * (16 * (D + 2) * 4 + kSpMaxParts * (int)sizeof(PartWeight))
-             ? kSoWarps * STAGES * 2 * kSoTile * D * 2 : kSoWarps * (16 * (D + 2) * 4 + kSpMaxParts * (int)sizeof(PartWeight));
+constexpr int own_smem(int per) {
+  const int tiles = kSoWarps * STAGES * 2 * kSoTile * D * 2, parts = kSoWarps * (per * (D + 2) * 4 + kSpMaxParts * (int)sizeof(PartWeight));
+  return tiles > parts ? tiles : parts;
 }
 
+// STAGES: tiles of a warp on their way or in use.  With a history most positions behind the prefix are common to a group, few are
+// left to a row, and what counts is how many rows are under way: one stage, four blocks on an SM (62 us against 67 for 16 groups of 4,
+// 113 against 119 for 4 of 16).  Without one all of them are the rows' own: two stages, three blocks (58 us against 73 for 48 rows
+// with up to 700).
 template <int D, int STAGES>
-__global__ void __launch_bounds__(kSoWarps * 32)
+__global__ void __launch_bounds__(kSoWarps * 32, STAGES == 1 ? 4 : 3)
 shared_own_kernel(const __grid_constant__ SharedParams p, const __grid_constant__ SharedPlan s) {
   constexpr int CH = D / 8;                       // 16-byte chunks per row
   constexpr int TILE_BYTES = kSoTile * D * 2;
@@ -983,24 +990,24 @@ shared_own_kernel(const __grid_constant__ SharedParams p, const __grid_constant_
     l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
   }
   __syncthreads();
-  float* so = reinterpret_cast<float*>(smem);                  // [warps][16][D]
-  float* sml = so + kSoWarps * 16 * D;                         // [warps][16][2]
+  float* so = reinterpret_cast<float*>(smem);                  // [warps][query heads][D]
+  float* sml = so + kSoWarps * per * D;                        // [warps][query heads][2]
 #pragma unroll
   for (int i2 = 0; i2 < D / 8; ++i2) {
     const int col = i2 * 8 + 2 * t4;
-    *reinterpret_cast<float2*>(so + ((size_t)warp * 16 + gi) * D + col) = make_float2(o[i2][0], o[i2][1]);
-    *reinterpret_cast<float2*>(so + ((size_t)warp * 16 + gi + 8) * D + col) = make_float2(o[i2][2], o[i2][3]);
+    if (gi < per) *reinterpret_cast<float2*>(so + (warp * per + gi) * D + col) = make_float2(o[i2][0], o[i2][1]);
+    if (gi + 8 < per) *reinterpret_cast<float2*>(so + (warp * per + gi + 8) * D + col) = make_float2(o[i2][2], o[i2][3]);
   }
   if (t4 == 0) {
-    *reinterpret_cast<float2*>(sml + (warp * 16 + gi) * 2) = make_float2(m_run[0], l_run[0]);
-    *reinterpret_cast<float2*>(sml + (warp * 16 + gi + 8) * 2) = make_float2(m_run[1], l_run[1]);
+    if (gi < per) *reinterpret_cast<float2*>(sml + (warp * per + gi) * 2) = make_float2(m_run[0], l_run[0]);
+    if (gi + 8 < per) *reinterpret_cast<float2*>(sml + (warp * per + gi + 8) * 2) = make_float2(m_run[1], l_run[1]);
   }
   __syncthreads();
   if (shared) pdl_wait();             // the shared positions' parts are there; and whoever waits for this kernel waits for that one
   if (p.n_own == 1) {
-    PartWeight* w = reinterpret_cast<PartWeight*>(sml + kSoWarps * 16 * 2) + warp * kSpMaxParts;
+    PartWeight* w = reinterpret_cast<PartWeight*>(sml + kSoWarps * per * 2) + warp * kSpMaxParts;
     for (int j = warp; j < per; j += kSoWarps) {
-      const OwnParts own = {sml + j * 2, so + j * D, kSoWarps, 16 * 2, 16 * D};
+      const OwnParts own = {sml + j * 2, so + j * D, kSoWarps, per * 2, per * D};
       add_parts<D>(p, s, gp, shared && in_group, row, hkv, j, own, w, lane);
     }
     return;
@@ -1009,14 +1016,14 @@ shared_own_kernel(const __grid_constant__ SharedParams p, const __grid_constant_
     const int r = idx / D, col = idx % D;
     float m_all = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kSoWarps; ++w) m_all = fmaxf(m_all, sml[(w * 16 + r) * 2]);
+    for (int w = 0; w < kSoWarps; ++w) m_all = fmaxf(m_all, sml[(w * per + r) * 2]);
     float acc = 0.0f, l_all = 0.0f;
 #pragma unroll
     for (int w = 0; w < kSoWarps; ++w) {
-      const float mw = sml[(w * 16 + r) * 2];
+      const float mw = sml[(w * per + r) * 2];
       const float f = (mw == -INFINITY) ? 0.0f : exp2f(mw - m_all);
-      acc += so[((size_t)w * 16 + r) * D + col] * f;
-      l_all += sml[(w * 16 + r) * 2 + 1] * f;
+      acc += so[(w * per + r) * D + col] * f;
+      l_all += sml[(w * per + r) * 2 + 1] * f;
     }
     const size_t at = ((size_t)row * p.n_q_heads + (size_t)hkv * per + r) * p.n_own + split;
     if (l_all > 0.0f) s.own_o[at * D + col] = acc;
@@ -1086,11 +1093,11 @@ template <int D>
 static int launch_tc(const SharedParams& p, int sms, cudaStream_t stream) {
   long long floats = 0;
   const SharedPlan s = layout(p, sms, &floats);
-  constexpr int STAGES = 2;
+  const int stages = p.history != nullptr ? 1 : 2;
   constexpr int smem_shared = 2 * kSpBM * D * 2 + 2 * kSpStages * kSpBN * D * 2 + 1024 + 512;
   static_assert(smem_shared + kSpSegments * sizeof(Segment) + 64 <= 232448, "shared memory of one block");
   static_assert((4 * kSpStages + 18) * 8 + 16 <= 512, "barriers");
-  constexpr int smem_own = own_smem<D, STAGES>();
+  const int per = p.n_q_heads / p.n_kv_heads, smem_own = stages == 1 ? own_smem<D, 1>(per) : own_smem<D, 2>(per);
   static bool configured[64] = {false};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1099,7 +1106,9 @@ static int launch_tc(const SharedParams& p, int sms, cudaStream_t stream) {
   if (!configured[dev]) {
     e = cudaFuncSetAttribute(shared_prefix_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_shared);
     if (e != cudaSuccess) return (int)e;
-    e = cudaFuncSetAttribute(shared_own_kernel<D, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_own);
+    e = cudaFuncSetAttribute(shared_own_kernel<D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, own_smem<D, 1>(16));
+    if (e != cudaSuccess) return (int)e;
+    e = cudaFuncSetAttribute(shared_own_kernel<D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, own_smem<D, 2>(16));
     if (e != cudaSuccess) return (int)e;
     configured[dev] = true;
   }
@@ -1126,7 +1135,7 @@ static int launch_tc(const SharedParams& p, int sms, cudaStream_t stream) {
     e = launch(shared_prefix_kernel<D>, dim3(s.blocks), dim3(kSpThreads), smem_shared, stream, mq, mk, mv, p, s);
     if (e != cudaSuccess) return (int)e;
   }
-  e = launch(shared_own_kernel<D, STAGES>, dim3(p.n_own, p.n_kv_heads, p.n_rows), dim3(kSoWarps * 32), smem_own, stream, p, s);
+  e = launch(stages == 1 ? shared_own_kernel<D, 1> : shared_own_kernel<D, 2>, dim3(p.n_own, p.n_kv_heads, p.n_rows), dim3(kSoWarps * 32), smem_own, stream, p, s);
   if (e != cudaSuccess || p.n_own == 1) return (int)e;
   const long long pairs = (long long)p.n_rows * p.n_q_heads;
   return (int)launch(shared_add_kernel<D>, dim3((unsigned)((pairs + kSmWarps - 1) / kSmWarps)), dim3(kSmWarps * 32), 0, stream, p, s);
