@@ -45,7 +45,7 @@ constexpr int kSpMinTiles = 3;        // tiles of a block, where there are so ma
 constexpr int kSpSegments = 32;       // pieces of triples that a block lists at a time
 
 // ---- plan ------------------------------------------------------------------------------------------------------------------
-constexpr int kPlanHead = 8, kPlanRecord = 8, kPlanThreads = 1024, kPlanGroups = 128;
+constexpr int kPlanHead = 8, kPlanRecord = 8, kPlanThreads = 1024, kPlanGroups = 64, kPlanMembers = 64;
 // head: 0 tiles in all, 1 blocks that take part.  A group's record: 0 first row, 1 members, 2 lowest visible position, 3 last visible
 // position of the prefix (< 2: none), 4 key tiles of the prefix, 5 first position of the common ones behind it, 6 one past their
 // last (where each member's own begin), 7 tiles of all groups before this one
@@ -76,7 +76,10 @@ __device__ __forceinline__ int plan_row_tiles(const GroupPlan& g, int members_pe
 
 __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_constant__ SharedParams p, const __grid_constant__ SharedPlan s) {
   pdl_trigger();
-  __shared__ int s_common[kPlanGroups], s_first[kPlanGroups], s_lo[kPlanGroups], s_hi[kPlanGroups];
+  // what is looked up once stays here: the kernels behind this one wait for it, and a load after another is most of its time
+  __shared__ int s_common[kPlanGroups], s_first[kPlanGroups], s_lo[kPlanGroups], s_hi[kPlanGroups], s_prefix[kPlanGroups];
+  __shared__ int2 s_rows[kPlanGroups];
+  __shared__ int s_slot[kPlanGroups][kPlanMembers];          // of the first members
   constexpr int WARPS = kPlanThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int carry = 0;                                             // warp 0: tiles of the groups so far
@@ -87,14 +90,15 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
     for (int k = warp; k < n_here; k += WARPS) {
       const int g = g0 + k;
       const int2 rows = group_rows(p, g);
-      const int prefix = max(0, p.prefix_len[g]);
+      const int prefix = max(0, p.prefix_len[g]), prefix_slot = p.prefix_slot[g];
       int lo = 0x7fffffff, last = -1, first = 0x7fffffff, bad = 0;
       for (int i = rows.x + lane; i < rows.y; i += 32) {
+        const int slot = p.req_slot[i];
+        if (slot < 0 || slot >= p.max_slots) bad = 1;
+        if (i - rows.x < kPlanMembers) s_slot[k][i - rows.x] = slot;
         const RowSpan sp = row_span(p, i);
         if (sp.pos < 0) { bad = 1; continue; }
         lo = min(lo, sp.lo); last = max(last, sp.pos); first = min(first, sp.pos);
-        const int slot = p.req_slot[i];
-        if (slot < 0 || slot >= p.max_slots) bad = 1;
       }
       lo = __reduce_min_sync(0xffffffffu, lo);
       last = __reduce_max_sync(0xffffffffu, last);
@@ -102,8 +106,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
       bad = __reduce_or_sync(0xffffffffu, (unsigned)bad);
       if (lane == 0) {
         int hi = min(prefix - 1, last);
-        if (hi >= lo && checked_slot(p, p.prefix_slot[g], rows.x) < 0) hi = -1;
-        s_lo[k] = lo; s_hi[k] = hi;
+        if (hi >= lo && checked_slot(p, prefix_slot, rows.x) < 0) hi = -1;
+        s_lo[k] = lo; s_hi[k] = hi; s_prefix[k] = prefix; s_rows[k] = rows;
         // positions behind the prefix and in front of every member's own, for which there are writers
         s_first[k] = p.history != nullptr && rows.y > rows.x && !bad ? max(0, min(first - prefix, p.history_ld)) : 0;
         s_common[k] = s_first[k];
@@ -115,26 +119,23 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
       const bool wide = p.history_ld % 16 == 0 && ((uintptr_t)p.history & 15) == 0;
       for (int pair = warp; pair < n_here * p.max_members; pair += WARPS) {
         const int k = pair / p.max_members, i = pair % p.max_members;
-        const int2 rows = group_rows(p, g0 + k);
+        const int2 rows = s_rows[k];
         const int n = rows.y - rows.x, most = s_first[k];
         if (i >= n || most == 0) continue;
-        const unsigned char* h0 = p.history + (size_t)p.req_slot[rows.x] * p.history_ld;
-        const unsigned char* h = p.history + (size_t)p.req_slot[rows.x + i] * p.history_ld;
+        const unsigned char* h0 = p.history + (size_t)s_slot[k][0] * p.history_ld;
+        const unsigned char* h = p.history + (size_t)(i < kPlanMembers ? s_slot[k][i] : p.req_slot[rows.x + i]) * p.history_ld;
         int common = most;
         if (wide) {
 #pragma unroll 2
           for (int c = lane; 16 * c < most; c += 32) {
             const uint4 x = *reinterpret_cast<const uint4*>(h0 + 16 * c), y = *reinterpret_cast<const uint4*>(h + 16 * c);
-            const unsigned int w[4] = {x.x, x.y, x.z, x.w}, d[4] = {x.x ^ y.x, x.y ^ y.y, x.z ^ y.z, x.w ^ y.w};
+            // a byte of the first member's row is looked at for its value, the others' for being the same
+            const unsigned int limit = (unsigned int)min(n, 255) * 0x01010101u;
+            const unsigned int w[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              // a byte of the first member's row is looked at for its value, the others' for being the same
-              if (i == 0) {
-#pragma unroll
-                for (int e = 3; e >= 0; --e) if ((int)((w[q] >> (8 * e)) & 255u) >= n) common = min(common, 16 * c + 4 * q + e);
-              } else if (d[q] != 0u) {
-                common = min(common, 16 * c + 4 * q + ((__ffs((int)d[q]) - 1) >> 3));
-              }
+            for (int q = 3; q >= 0; --q) {
+              const unsigned int off = i > 0 ? w[q] ^ v[q] : n <= 255 ? __vcmpgeu4(w[q], limit) : 0u;
+              if (off != 0u) common = min(common, 16 * c + 4 * q + ((__ffs((int)off) - 1) >> 3));
             }
           }
         } else {
@@ -153,8 +154,8 @@ __global__ void __launch_bounds__(kPlanThreads) shared_plan_kernel(const __grid_
         int v = 0;
         GroupPlan gp = {};
         if (k < n_here) {
-          const int2 rows = group_rows(p, g);
-          const int prefix = max(0, p.prefix_len[g]), lo = s_lo[k], hi = s_hi[k], end = prefix + s_common[k];
+          const int2 rows = s_rows[k];
+          const int prefix = s_prefix[k], lo = s_lo[k], hi = s_hi[k], end = prefix + s_common[k];
           gp = {rows.x, rows.y - rows.x, lo, hi, hi >= lo ? hi / kSpBN - lo / kSpBN + 1 : 0, max(prefix, min(lo, end)), end, 0};
           v = plan_tiles(gp) * plan_row_tiles(gp, s.members_per_tile) * p.n_kv_heads;
         }

@@ -2033,13 +2033,15 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     _want_here((q, kind, "q"), (out, kind, "out"), (k_cache, kind, "k_cache"), (v_cache, kind, "v_cache"), (positions, i32, "positions"),
                (req_slot, i32, "req_slot"), (block_table, i32, "block_table"), (err, i32, "err"),
                (shared.group_start, i32, "group_start"), (shared.prefix_slot, i32, "prefix_slot"), (shared.prefix_len, i32, "prefix_len"))
-    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4 or block_table.dim() != 2:
+    qs, ks, vs, ts = q.shape, k_cache.shape, v_cache.shape, block_table.shape
+    if len(qs) != 3 or len(ks) != 4 or len(vs) != 4 or len(ts) != 2:
         raise KernelError("q must be [rows, Hq, d], the caches [pages, Hkv, page, d], the block table [slots, pages]")
-    rows, hq, d = q.shape
-    num_pages, hkv, page_size, dk = k_cache.shape
-    dv = v_cache.shape[3]
+    rows, hq, d = qs
+    num_pages, hkv, page_size, dk = ks
+    dv = vs[3]
+    slots, max_pages = ts
     groups = shared.prefix_len.numel()
-    if dk != d or tuple(v_cache.shape[:3]) != (num_pages, hkv, page_size) or tuple(out.shape) != (rows, hq, dv):
+    if dk != d or vs != (num_pages, hkv, page_size, dv) or out.shape != (rows, hq, dv):
         raise KernelError(f"queries {tuple(q.shape)}, caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} and output "
                           f"{tuple(out.shape)} do not fit")
     if hkv < 1 or hq % hkv or d > 256 or dv > 256:
@@ -2056,7 +2058,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     history, ld = shared.history, 0
     if history is not None:
         _want_here((history, torch.uint8, "history"))
-        if history.dim() != 2 or history.shape[0] != block_table.shape[0]:
+        if history.dim() != 2 or history.shape[0] != slots:
             raise KernelError("history must be [slots, n] for the slots of the block table")
         if shared.max_members > 256:
             raise KernelError(f"a history names up to 256 members of a group, got {shared.max_members}")
@@ -2073,9 +2075,8 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     scratch = torch.empty(need, dtype=torch.float32, device=q.device)
     _check(_lib().tk_attention_shared(*ptrs, shared.group_start.data_ptr(), shared.prefix_slot.data_ptr(), shared.prefix_len.data_ptr(),
                                       positions.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), _ptr(history), _ptr(sinks),
-                                      scratch.data_ptr(), err.data_ptr(), *sizes, block_table.shape[1], num_pages, block_table.shape[0],
-                                      ld, window or 0, n_shared, n_own, scale, softcap or 0.0, dtype, _stream()),
-           "attention_shared")
+                                      scratch.data_ptr(), err.data_ptr(), *sizes, max_pages, num_pages, slots, ld, window or 0, n_shared,
+                                      n_own, scale, softcap or 0.0, dtype, _stream()), "attention_shared")
 
 
 def sm_count(device: torch.device) -> int:
