@@ -124,6 +124,17 @@ def test_selection(groups, beams, vocab, k, kind):
     check_selection(x, s, k, got)
 
 
+@pytest.mark.parametrize("kind", ["normal", "rising", "few_values", "far"])
+@pytest.mark.parametrize("k", [8, 256])
+def test_selection_in_long_segments(k, kind):
+    """Rows enough for one segment each: many tiles between the first threshold and the last."""
+    x, s = select_inputs(kind, 145, 4, 60007, seed=3)
+    got = ops.beam_select(torch.from_numpy(x).to(DEV), torch.from_numpy(s).to(DEV), k)
+    some = slice(0, 2)                           # the oracle sorts every group: the first two and the last
+    check_selection(x[:8], s[some], k, tuple(t[some] for t in got))
+    check_selection(x[-4:], s[-1:], k, tuple(t[-1:] for t in got))
+
+
 @pytest.mark.parametrize("offset,extra", [(0, 1), (1, 0), (2, 5), (3, 2)])
 def test_selection_of_rows_that_start_on_any_four_bytes(offset, extra):
     groups, beams, vocab, k = 2, 3, 9973, 12
@@ -562,6 +573,23 @@ def test_shared_attention_of_keys_that_come_late(d):
         x.out.fill_(float("nan"))
         assert torch.equal(x.call(), first), f"call {i}"
     x.check()
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("prefixes,window", [([70, 0], None), ([0, 0], None), ([300, 33], 700)])
+def test_shared_attention_of_long_own_positions(prefixes, window, dtype, d):
+    """Few rows with many positions of their own, which several blocks share out."""
+    c = Shared([2, 1], prefixes, [900, 530, 257], hq=8, hkv=2, d=d, dtype=dtype, window=window, sinks=True, seed=21).device()
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("history", [False, True])
+def test_shared_attention_of_groups_without_members(history, dtype):
+    c = Shared([0, 2, 0, 0, 3, 0], [40, 70, 0, 130, 200, 65], 30, d=64, dtype=dtype, history=history, seed=22).device()
+    c.call()
+    c.check()
 
 
 def test_shared_attention_at_addresses_on_any_boundary():

@@ -34,7 +34,7 @@ struct SharedParams {
   const float* sinks;           // [n_q_heads] or null
   float* part_o;                // [rows, n_q_heads, n_parts, dv]   (the general kernel's)
   float* part_ml;               // [rows, n_q_heads, n_parts, 2]
-  float* scratch;               // 16-byte aligned
+  float* scratch;               // 32-byte aligned
   int* err;
   int n_rows, n_groups, max_members, n_q_heads, n_kv_heads, d, dv, page_size, max_pages, num_pages, max_slots, history_ld, window;
   int n_shared, n_own, n_parts; // parts of the shared and of the other positions; n_parts = n_shared + n_own
@@ -102,7 +102,10 @@ __device__ __forceinline__ bool row_has_group(const SharedParams& p, int row, in
 struct RowSpan { int pos, lo; };
 __device__ __forceinline__ RowSpan row_span(const SharedParams& p, int row) {
   const int pos = p.positions[row];
-  if (pos < 0) { set_error(p.err, kErrPosition, row, pos, 0); return {-1, 0}; }
+  if (pos < 0 || pos >= (long long)p.max_pages * p.page_size) {          // none, or one that the block table has no place for
+    set_error(p.err, kErrPosition, row, pos, p.max_pages);
+    return {-1, 0};
+  }
   return {pos, first_visible(pos, p.window, 0)};
 }
 

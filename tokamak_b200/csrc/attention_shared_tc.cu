@@ -1097,6 +1097,9 @@ template <int D>
 static int launch_tc(const SharedParams& p, int sms, cudaStream_t stream) {
   long long floats = 0;
   const SharedPlan s = layout(p, sms, &floats);
+  // the key tiles of all triples are counted in 32 bits
+  const long long triples = (long long)p.n_kv_heads * (p.n_groups + (has_shared(p) ? p.n_rows / (2 * s.members_per_tile) : 0));
+  if (triples * ((long long)p.max_pages * p.page_size / kSpBN + 3) > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
   const int stages = p.history != nullptr ? 1 : 2;
   constexpr int smem_shared = 2 * kSpBM * D * 2 + 2 * kSpStages * kSpBN * D * 2 + 1024 + 512;
   static_assert(smem_shared + kSpSegments * sizeof(Segment) + 64 <= 232448, "shared memory of one block");

@@ -763,12 +763,6 @@ __global__ void __launch_bounds__(kMoveThreads) reorder_slots_kernel(const __gri
 
 }  // namespace tk
 
-TK_API int tk_beam_select_tile(void) { return tk::kSelTile; }
-TK_API int tk_beam_max_beams(void) { return tk::kSelMaxBeams; }
-TK_API int tk_beam_max_candidates(void) { return tk::kSelMaxK; }
-TK_API int tk_beam_max_entries(void) { return tk::kSelMaxEntries; }
-TK_API int tk_reorder_max_tensors(void) { return tk::kMoveMaxTensors; }
-
 // scratch: rows * segments * (16 + 8 k) bytes, on 8 bytes.
 TK_API int tk_beam_select(const float* logits, long long ld, const float* scores, void* scratch, float* out_scores,
                           int* out_parents, int* out_tokens, int groups, int beams, int vocab, int k, int segments,

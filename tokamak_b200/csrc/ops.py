@@ -2000,15 +2000,21 @@ def shared_splits(sms: int, groups: int, rows: int, n_q_heads: int, n_kv_heads: 
     return n_shared, max(1, min(2 * sms // max(1, rows * n_kv_heads), -(-own // 32)))
 
 
+_SHARED_MAX_OWN = 16              # parts of a row's own positions that the tensor-core kernel adds up
+
+
 @lru_cache(maxsize=1024)
 def _shared_plan(sms: int, sizes: tuple, num_pages: int, max_prefix: int, max_own: int, window: int, has_history: bool, at: int,
                  out_at: int, dtype: int) -> tuple[int, int, int]:
     """Parts of the shared and the other positions, and the floats of scratch, of a call of these sizes; ``at`` and ``out_at``: where
-    its tensors begin within 16 bytes.  The tensor-core kernel deals its work out itself; what counts for it is whether
-    anything is shared."""
+    its tensors begin within 16 bytes.  The tensor-core kernel deals the shared positions out itself; what counts for it is whether
+    there are any.  A row's own ones, of which a history leaves few, are cut into parts of 256 or more while three blocks an SM
+    are free (2 rows with 1,024 of their own behind 4,096: 29 us instead of 43; 32 rows, of which each gets one block, would
+    take 55 with two instead of 49)."""
     rows, groups, members, hq, hkv, d, dv, page_size = sizes
     if dtype == 1 and shared_tc_takes(hq, hkv, d, dv, page_size):
-        n_shared, n_own = int(max_prefix > 0), 1
+        own = min(max_own, window) if window else max_own
+        n_shared, n_own = int(max_prefix > 0), 1 if has_history else max(1, min(_SHARED_MAX_OWN, 3 * sms // max(1, rows * hkv), own // 256))
     else:
         n_shared, n_own = shared_splits(sms, groups, rows, hq, hkv, members, max_prefix, max_own, window)
     need = library().tk_attention_shared_scratch(at, out_at, at, at, int(has_history) or None, *sizes, num_pages, n_shared, n_own, dtype)
@@ -2075,8 +2081,8 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     scratch = torch.empty(need, dtype=torch.float32, device=q.device)
     _check(_lib().tk_attention_shared(*ptrs, shared.group_start.data_ptr(), shared.prefix_slot.data_ptr(), shared.prefix_len.data_ptr(),
                                       positions.data_ptr(), req_slot.data_ptr(), block_table.data_ptr(), _ptr(history), _ptr(sinks),
-                                      scratch.data_ptr(), err.data_ptr(), *sizes, max_pages, num_pages, slots, ld, window or 0, n_shared,
-                                      n_own, scale, softcap or 0.0, dtype, _stream()), "attention_shared")
+                                      scratch.data_ptr(), err.data_ptr(), *sizes, max_pages, num_pages, slots, ld, int(window or 0), n_shared,
+                                      n_own, float(scale), float(softcap or 0.0), dtype, _stream()), "attention_shared")
 
 
 def sm_count(device: torch.device) -> int:
