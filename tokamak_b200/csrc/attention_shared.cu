@@ -16,22 +16,39 @@ constexpr int kShRows = 32;
 constexpr int kShKeys = 32;
 constexpr int kShThreads = 256;
 
+// Four elements as floats.
 template <typename T>
-__device__ __forceinline__ void load_row(float* dst, const T* src, int n, bool wide, int lane0, int lanes) {
-  if (wide) {
-    for (int c = lane0; c < n / 4; c += lanes) {
-      float4 f;
-      if constexpr (sizeof(T) == 4) {
-        f = *reinterpret_cast<const float4*>(src + 4 * c);
+__device__ __forceinline__ float4 load4(const T* src) {
+  if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float4*>(src);
+  const uint2 u = *reinterpret_cast<const uint2*>(src);
+  const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&u.x), b = *reinterpret_cast<const __nv_bfloat162*>(&u.y);
+  return make_float4(__bfloat162float(a.x), __bfloat162float(a.y), __bfloat162float(b.x), __bfloat162float(b.y));
+}
+
+// N rows of n elements each to shared memory by a warp, padded with zeros to a multiple of four; src(r) is null for a row of
+// zeros, dst(r) null for none.  The rows' loads are under way together.
+template <typename T, int N, typename Src, typename Dst>
+__device__ __forceinline__ void load_rows(int n, bool wide, int lane, Src src, Dst dst) {
+  for (int c = lane; c < (n + 3) / 4; c += 32) {
+    float4 f[N];
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+      const T* from = src(r);
+      f[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (from == nullptr) continue;
+      if (wide) {
+        f[r] = load4<T>(from + 4 * c);
       } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(src + 4 * c);
-        const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&u.x), b = *reinterpret_cast<const __nv_bfloat162*>(&u.y);
-        f = make_float4(__bfloat162float(a.x), __bfloat162float(a.y), __bfloat162float(b.x), __bfloat162float(b.y));
+        float* e = &f[r].x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) if (4 * c + k < n) e[k] = to_f32<T>(from[4 * c + k]);
       }
-      *reinterpret_cast<float4*>(dst + 4 * c) = f;
     }
-  } else {
-    for (int c = lane0; c < n; c += lanes) dst[c] = to_f32<T>(src[c]);
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+      float* to = dst(r);
+      if (to != nullptr) *reinterpret_cast<float4*>(to + 4 * c) = f[r];
+    }
   }
 }
 
@@ -103,10 +120,11 @@ __global__ void __launch_bounds__(kShThreads) shared_parts_kernel(SharedParams p
 
   const bool wide_k = p.wide_k, wide_v = p.wide_v;
   if (t0 < t1) {
-    for (int i = warp; i < n_pairs; i += kShThreads / 32) {
-      load_row<T>(s_q + i * dp, (const T*)p.q + ((size_t)s_tok[i] * p.n_q_heads + s_head[i]) * p.d, p.d, wide_k, lane, 32);
-      for (int c = p.d + lane; c < dp; c += 32) s_q[i * dp + c] = 0.0f;
-    }
+    constexpr int WARPS = kShThreads / 32;
+    load_rows<T, kShRows / WARPS>(p.d, wide_k, lane, [&](int r) -> const T* {
+      const int i = warp + r * WARPS;
+      return i < n_pairs ? (const T*)p.q + ((size_t)s_tok[i] * p.n_q_heads + s_head[i]) * p.d : nullptr;
+    }, [&](int r) -> float* { return warp + r * WARPS < n_pairs ? s_q + (warp + r * WARPS) * dp : nullptr; });
   }
   float m[4], l[4], acc[4][4 * kChunks];
 #pragma unroll
@@ -129,23 +147,24 @@ __global__ void __launch_bounds__(kShThreads) shared_parts_kernel(SharedParams p
       s_row[tid] = at;
     }
     __syncthreads();
-    for (int i = warp; i < kShKeys; i += kShThreads / 32) {
-      const long long at = s_row[i];
-      if (at >= 0) {
-        load_row<T>(s_k + i * ldk, (const T*)p.k_cache + at * p.d, p.d, wide_k, lane, 32);
-        load_row<T>(s_v + i * dvp, (const T*)p.v_cache + at * p.dv, p.dv, wide_v, lane, 32);
-        for (int c = p.d + lane; c < dp; c += 32) s_k[i * ldk + c] = 0.0f;
-      } else {
-        // a key that is not there: nothing that lies in its place may reach the result
-        for (int c = lane; c < dp; c += 32) s_k[i * ldk + c] = 0.0f;
-        for (int c = lane; c < dvp; c += 32) s_v[i * dvp + c] = 0.0f;
-      }
+    {
+      // (a key that is not there is zeros: nothing that lies in its place may reach the result)
+      constexpr int WARPS = kShThreads / 32, N = kShKeys / WARPS;
+      load_rows<T, N>(p.d, wide_k, lane, [&](int r) -> const T* {
+        const long long at = s_row[warp + r * WARPS];
+        return at >= 0 ? (const T*)p.k_cache + at * p.d : nullptr;
+      }, [&](int r) { return s_k + (warp + r * WARPS) * ldk; });
+      load_rows<T, N>(p.dv, wide_v, lane, [&](int r) -> const T* {
+        const long long at = s_row[warp + r * WARPS];
+        return at >= 0 ? (const T*)p.v_cache + at * p.dv : nullptr;
+      }, [&](int r) { return s_v + (warp + r * WARPS) * dvp; });
     }
     __syncthreads();
     if (active) {
       float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       const float* kr = s_k + lane * ldk;
       const float* qr = s_q + 4 * warp * dp;
+#pragma unroll 4
       for (int c = 0; c < dp; c += 4) {
         const float4 kv = *reinterpret_cast<const float4*>(kr + c);
 #pragma unroll
@@ -178,6 +197,7 @@ __global__ void __launch_bounds__(kShThreads) shared_parts_kernel(SharedParams p
       for (int ch = 0; ch < kChunks; ++ch) {
         const int col = ch * 128 + lane * 4;
         if (col < dvp) {
+#pragma unroll 8
           for (int j = 0; j < kShKeys; ++j) {
             const float4 w = *reinterpret_cast<const float4*>(&s_p[warp][j][0]);
             const float4 vv = *reinterpret_cast<const float4*>(s_v + j * dvp + col);
