@@ -25,29 +25,29 @@ __device__ __forceinline__ float4 load4(const T* src) {
   return make_float4(__bfloat162float(a.x), __bfloat162float(a.y), __bfloat162float(b.x), __bfloat162float(b.y));
 }
 
-// N rows of n elements each to shared memory by a warp, padded with zeros to a multiple of four; src(r) is null for a row of
-// zeros, dst(r) null for none.  The rows' loads are under way together.
-template <typename T, int N, typename Src, typename Dst>
-__device__ __forceinline__ void load_rows(int n, bool wide, int lane, Src src, Dst dst) {
-  for (int c = lane; c < (n + 3) / 4; c += 32) {
+// N rows of len(r) elements, `longest` at most, to shared memory by a warp, padded with zeros to a multiple of four; src(r) is null
+// for a row of zeros, dst(r) null for none.  The rows' loads are under way together.
+template <typename T, int N, typename Len, typename Src, typename Dst>
+__device__ __forceinline__ void load_rows(int longest, bool wide, int lane, Len len, Src src, Dst dst) {
+  for (int c = 4 * lane; c < longest; c += 128) {
     float4 f[N];
 #pragma unroll
     for (int r = 0; r < N; ++r) {
       const T* from = src(r);
       f[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (from == nullptr) continue;
+      if (from == nullptr || c >= len(r)) continue;
       if (wide) {
-        f[r] = load4<T>(from + 4 * c);
+        f[r] = load4<T>(from + c);
       } else {
         float* e = &f[r].x;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) if (4 * c + k < n) e[k] = to_f32<T>(from[4 * c + k]);
+        for (int k = 0; k < 4; ++k) if (c + k < len(r)) e[k] = to_f32<T>(from[c + k]);
       }
     }
 #pragma unroll
     for (int r = 0; r < N; ++r) {
       float* to = dst(r);
-      if (to != nullptr) *reinterpret_cast<float4*>(to + 4 * c) = f[r];
+      if (to != nullptr && c < len(r)) *reinterpret_cast<float4*>(to + c) = f[r];
     }
   }
 }
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kShThreads) shared_parts_kernel(SharedParams p
   const bool wide_k = p.wide_k, wide_v = p.wide_v;
   if (t0 < t1) {
     constexpr int WARPS = kShThreads / 32;
-    load_rows<T, kShRows / WARPS>(p.d, wide_k, lane, [&](int r) -> const T* {
+    load_rows<T, kShRows / WARPS>(p.d, wide_k, lane, [&](int) { return p.d; }, [&](int r) -> const T* {
       const int i = warp + r * WARPS;
       return i < n_pairs ? (const T*)p.q + ((size_t)s_tok[i] * p.n_q_heads + s_head[i]) * p.d : nullptr;
     }, [&](int r) -> float* { return warp + r * WARPS < n_pairs ? s_q + (warp + r * WARPS) * dp : nullptr; });
@@ -150,14 +150,10 @@ __global__ void __launch_bounds__(kShThreads) shared_parts_kernel(SharedParams p
     {
       // (a key that is not there is zeros: nothing that lies in its place may reach the result)
       constexpr int WARPS = kShThreads / 32, N = kShKeys / WARPS;
-      load_rows<T, N>(p.d, wide_k, lane, [&](int r) -> const T* {
-        const long long at = s_row[warp + r * WARPS];
-        return at >= 0 ? (const T*)p.k_cache + at * p.d : nullptr;
-      }, [&](int r) { return s_k + (warp + r * WARPS) * ldk; });
-      load_rows<T, N>(p.dv, wide_v, lane, [&](int r) -> const T* {
-        const long long at = s_row[warp + r * WARPS];
-        return at >= 0 ? (const T*)p.v_cache + at * p.dv : nullptr;
-      }, [&](int r) { return s_v + (warp + r * WARPS) * dvp; });
+      load_rows<T, 2 * N>(max(p.d, p.dv), wide_k && wide_v, lane, [&](int r) { return r < N ? p.d : p.dv; }, [&](int r) -> const T* {
+        const long long at = s_row[warp + r % N * WARPS];
+        return at < 0 ? nullptr : r < N ? (const T*)p.k_cache + at * p.d : (const T*)p.v_cache + at * p.dv;
+      }, [&](int r) { return r < N ? s_k + (warp + r * WARPS) * ldk : s_v + (warp + (r - N) * WARPS) * dvp; });
     }
     __syncthreads();
     if (active) {
