@@ -309,6 +309,36 @@ def test_records_follow(groups, seats, kind):
     assert err.tolist()[0] == 0
 
 
+@pytest.mark.parametrize("kind", ["identity", "shift", "random", "all_from_one", "in_two"])
+@pytest.mark.parametrize("groups,seats,sizes", [(3, 8, [(2, 400004), (1, 4), (3, 3076)]), (1, 24, [(5, 700000)]), (60, 16, [(2, 20488), (1, 12)]),
+                                                (200, 2, [(1, 16384)])])
+def test_long_records_follow(groups, seats, sizes, kind):
+    """Records of many bytes (sizes: keys, and floats of a record), among short ones."""
+    rng = np.random.default_rng(13)
+    max_slots = groups * seats + 3
+    slots = rng.permutation(max_slots)[:groups * seats].reshape(groups, seats)
+    parents = {"identity": np.tile(np.arange(seats), (groups, 1)), "shift": np.tile(np.roll(np.arange(seats), 1), (groups, 1)),
+               "random": rng.integers(0, seats, (groups, seats)), "all_from_one": np.full((groups, seats), seats - 1),
+               "in_two": np.where(rng.random((groups, 1)) < 0.5, np.arange(seats), np.arange(seats) // 2 * 2)}[kind]
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    tensors = [torch.randn(keys, max_slots, n, device=DEV, generator=gen) for keys, n in sizes]
+    at, source = torch.from_numpy(slots).to(DEV), torch.from_numpy(np.take_along_axis(slots, parents, axis=1)).to(DEV)
+    want = []
+    for t in tensors:
+        w = t.clone()
+        w[:, at.reshape(-1)] = t[:, source.reshape(-1)]
+        want.append(w)
+    err = err_word()
+    ops.reorder_slots(tensors, i32(slots), i32(parents), err)
+    assert all(torch.equal(a, b) for a, b in zip(tensors, want)) and err.tolist()[0] == 0
+    # a seat with a slot or a parent that there is not stays as it is, and so does what would go on from it
+    before = [t.clone() for t in tensors]
+    bad_slots, bad_parents = slots.copy(), np.tile(np.arange(seats), (groups, 1))
+    bad_slots[0, 0], bad_parents[0, 1], bad_parents[-1, 0] = max_slots, 0, seats
+    ops.reorder_slots(tensors, i32(bad_slots), i32(bad_parents), err)
+    assert all(torch.equal(a, b) for a, b in zip(tensors, before)) and err.tolist()[0] == 4
+
+
 def test_records_at_addresses_on_any_boundary_and_many_tensors():
     memory = torch.arange(0, 4096, dtype=torch.int32, device=DEV).to(torch.uint8)
     err = err_word()

@@ -10,8 +10,9 @@ namespace tk {
 // the pairs are those of a tile of the group's members, or of one row's others.  Tiles of 32 keys go through shared memory as
 // float32; warp w holds four pairs: a lane computes the four scores of its key, then owns four (or eight) columns of the output.
 // Bound by latency where it is used (float32, and shapes the tensor-core kernels refuse): 4 rows of 16 query heads over 8 of
-// 64, 1,021 shared and 61 further positions in float32 take 23 us, of which the keys' 4.5 MB would need one.  So the
-// keys are cut down to 32 a block, and both kinds of positions go into one launch (64 a block and two launches: 37 us).
+// 64, 1,021 shared and 61 further positions in float32 take 19 us, of which the keys' 4.5 MB would need one.  So the
+// keys are cut down to 32 a block, both kinds of positions go into one launch (64 a block and two launches: 37 us, 23 without
+// them), and a warp's loads of a tile are on their way together.
 constexpr int kShRows = 32;
 constexpr int kShKeys = 32;
 constexpr int kShThreads = 256;
