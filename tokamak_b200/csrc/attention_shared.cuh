@@ -37,7 +37,8 @@ struct SharedParams {
   float* scratch;               // 32-byte aligned
   int* err;
   int n_rows, n_groups, max_members, n_q_heads, n_kv_heads, d, dv, page_size, max_pages, num_pages, max_slots, history_ld, window;
-  int n_shared, n_own, n_parts; // parts of the shared and of the other positions; n_parts = n_shared + n_own
+  int n_shared, n_own, n_parts; // parts of the shared and of the other positions; n_parts = n_shared + n_own (on the tensor cores
+                                // n_shared is the number of blocks for the shared ones, 0: nothing is but by a history)
   int wide_k, wide_v;           // rows of queries and keys, of values, can be read four elements at a time
   float scale_log2, cap_log2, inv_cap;
 };

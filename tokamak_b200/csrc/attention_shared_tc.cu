@@ -32,7 +32,8 @@
 //
 // Other positions: mma.sync, a block per (range of keys, key/value head, row), the query heads over the key/value head as
 // the rows of a 16-row tile.  Four warps walk 16-key tiles with cp.async, each key's address looked up once, ahead of the
-// loop, for the block.  With one range to a row the block adds the shared parts up itself.
+// loop, for the block.  Where the shared positions get all SMs and a row is one range, the block adds the shared parts up itself;
+// otherwise the two kinds of positions run side by side and a third kernel does.
 #include "attention_shared.cuh"
 #include "tcgen05_utils.cuh"
 
@@ -56,6 +57,7 @@ struct SharedPlan {
   int* ints;
   int blocks;              // of the shared positions' kernel
   int members_per_tile;
+  bool apart;              // rows' own parts go to own_o and the parts are added up by a kernel of their own
   float* slot_o;           // [blocks][2 pieces][2 softmax groups][128 rows][D]
   float* slot_ml;          // [blocks][2][2][128][2]
   float* whole_o;          // [rows][n_q_heads][2][D]: triples that one block holds whole
@@ -1007,8 +1009,8 @@ shared_own_kernel(const __grid_constant__ SharedParams p, const __grid_constant_
     if (gi + 8 < per) *reinterpret_cast<float2*>(sml + (warp * per + gi + 8) * 2) = make_float2(m_run[1], l_run[1]);
   }
   __syncthreads();
-  if (shared) pdl_wait();             // the shared positions' parts are there; and whoever waits for this kernel waits for that one
-  if (p.n_own == 1) {
+  if (!s.apart) {
+    if (shared) pdl_wait();           // the shared positions' parts are there; and whoever waits for this kernel waits for that one
     PartWeight* w = reinterpret_cast<PartWeight*>(sml + kSoWarps * per * 2) + warp * kSpMaxParts;
     for (int j = warp; j < per; j += kSoWarps) {
       const OwnParts own = {sml + j * 2, so + j * D, kSoWarps, per * 2, per * D};
@@ -1033,9 +1035,11 @@ shared_own_kernel(const __grid_constant__ SharedParams p, const __grid_constant_
     if (l_all > 0.0f) s.own_o[at * D + col] = acc;
     if (col == 0) { s.own_ml[2 * at] = m_all; s.own_ml[2 * at + 1] = l_all; }
   }
+  // whoever waits for this kernel waits for the shared positions' one, for which one block that does is enough
+  if (shared && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) pdl_wait();
 }
 
-// Rows whose own positions several blocks shared out: a warp per (row, query head).
+// The parts of rows whose own ones were left apart: a warp per (row, query head).
 constexpr int kSmWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(kSmWarps * 32) shared_add_kernel(const __grid_constant__ SharedParams p, const __grid_constant__ SharedPlan s) {
@@ -1073,13 +1077,15 @@ static SharedPlan layout(const SharedParams& p, int sms, long long* floats) {
   if (has_shared(p)) {
     s.ints = reinterpret_cast<int*>(take(kPlanHead + (long long)p.n_groups * kPlanRecord));
     s.blocks = sms < kSpMaxBlocks ? sms : kSpMaxBlocks;
+    if (p.n_shared > 0 && p.n_shared < s.blocks) { s.blocks = p.n_shared; s.apart = true; }
     s.members_per_tile = kSpBM / (p.n_q_heads / p.n_kv_heads);
     s.slot_ml = take(4LL * s.blocks * kSpBM * 2);
     s.whole_ml = take(pairs * 2 * 2);
     s.slot_o = take(4LL * s.blocks * kSpBM * p.d);
     s.whole_o = take(pairs * 2 * p.d);
   }
-  if (p.n_own > 1) {
+  s.apart = s.apart || p.n_own > 1;
+  if (s.apart) {
     s.own_ml = take(pairs * p.n_own * 2);
     s.own_o = take(pairs * p.n_own * p.d);
   }
@@ -1143,7 +1149,7 @@ static int launch_tc(const SharedParams& p, int sms, cudaStream_t stream) {
     if (e != cudaSuccess) return (int)e;
   }
   e = launch(stages == 1 ? shared_own_kernel<D, 1> : shared_own_kernel<D, 2>, dim3(p.n_own, p.n_kv_heads, p.n_rows), dim3(kSoWarps * 32), smem_own, stream, p, s);
-  if (e != cudaSuccess || p.n_own == 1) return (int)e;
+  if (e != cudaSuccess || !s.apart) return (int)e;
   const long long pairs = (long long)p.n_rows * p.n_q_heads;
   return (int)launch(shared_add_kernel<D>, dim3((unsigned)((pairs + kSmWarps - 1) / kSmWarps)), dim3(kSmWarps * 32), 0, stream, p, s);
 }

@@ -2007,14 +2007,35 @@ _SHARED_MAX_OWN = 16              # parts of a row's own positions that the tens
 def _shared_plan(sms: int, sizes: tuple, num_pages: int, max_prefix: int, max_own: int, window: int, has_history: bool, at: int,
                  out_at: int, dtype: int) -> tuple[int, int, int]:
     """Parts of the shared and the other positions, and the floats of scratch, of a call of these sizes; ``at`` and ``out_at``: where
-    its tensors begin within 16 bytes.  The tensor-core kernel deals the shared positions out itself; what counts for it is whether
-    there are any.  A row's own ones, of which a history leaves few, are cut into parts of 256 or more while three blocks an SM
-    are free (2 rows with 1,024 of their own behind 4,096: 29 us instead of 43; 32 rows, of which each gets one block, would
-    take 55 with two instead of 49)."""
+    its tensors begin within 16 bytes.
+
+    The tensor-core kernel deals the shared positions out itself, to as many blocks as it is given, one an SM.  With a history
+    few of the other positions are left to a row: it gets all SMs, and what is left is done behind it.  Without one the rows'
+    own positions may be as much work.  They are cut into parts of 256 or more while three blocks an SM are free, and the SMs
+    that the shared ones are not given do them at the same time.  The shared ones get twice their tiles' share of all (the tiles
+    of more than 128 query rows count half as much again), ten tiles or more a block, and a product's tiles in equal parts.
+
+    With 32 query heads over 8 of 128: 48 rows, 8,192 shared positions, up to 700 of their own 47 us instead of 55; 32 rows in
+    two groups, 2,048 and 1,024, 39 instead of 49; 2 rows, 4,096 and 1,024, 21 instead of 44.  Where the shared positions need most
+    of the SMs anyway (64 rows in 16 groups, 4,093 and 129: 62 us with all, 65 with 128) or few of them (64 rows, 1,024 and
+    1,024: 52 us, 56 with 16), they get all they want."""
     rows, groups, members, hq, hkv, d, dv, page_size = sizes
     if dtype == 1 and shared_tc_takes(hq, hkv, d, dv, page_size):
-        own = min(max_own, window) if window else max_own
-        n_shared, n_own = int(max_prefix > 0), 1 if has_history else max(1, min(_SHARED_MAX_OWN, 3 * sms // max(1, rows * hkv), own // 256))
+        n_shared, n_own = sms if max_prefix > 0 else 0, 1
+        if not has_history:
+            prefix, own, rows_heads = max_prefix, max_own, max(1, rows * hkv)
+            if window:
+                prefix, own = min(prefix, window), min(own, window)
+            n_own = max(1, min(_SHARED_MAX_OWN, 3 * sms // rows_heads, own // 256))
+            row_tiles = -(-members * (hq // hkv) // 256)
+            products = groups * hkv * row_tiles
+            tiles = products * -(-prefix // 64)
+            if tiles > sms:
+                cost = tiles * (1.5 if members * (hq // hkv) > 128 else 1.0)
+                blocks = min(2 * cost / (cost + rows_heads * (own / 64 + 2)) * sms, tiles / 10)
+                if blocks > products:
+                    blocks = round(blocks / products) * products          # a product's tiles in as many equal parts
+                n_shared = sms if blocks > sms * 7 // 8 else max(16, int(blocks))
     else:
         n_shared, n_own = shared_splits(sms, groups, rows, hq, hkv, members, max_prefix, max_own, window)
     need = library().tk_attention_shared_scratch(at, out_at, at, at, int(has_history) or None, *sizes, num_pages, n_shared, n_own, dtype)
