@@ -591,6 +591,19 @@ def test_shared_attention_of_very_many_small_groups():
     c.check()
 
 
+@pytest.mark.parametrize("d,hkv", [(64, 2), (128, 2), (128, 8)])
+def test_shared_attention_of_groups_of_all_sizes(d, hkv):
+    """One tile of query rows and two, long sequences of keys and single tiles in turn."""
+    members, prefixes = [40, 1, 70, 3, 33, 2, 64, 1, 5], [700, 3, 310, 64, 129, 1, 500, 65, 260]
+    x = Shared(members, prefixes, own=24, hq=4 * hkv, hkv=hkv, d=d, history=True, common=20, seed=9).device()
+    first = x.call().clone()
+    x.check(first)
+    cold = torch.empty(1 << 28, dtype=torch.uint8, device=DEV)
+    for i in range(12):
+        cold.fill_(i)
+        assert torch.equal(x.call(), first), f"call {i}"
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_shared_attention_of_keys_that_come_late(d):
     """Long sequences of key tiles in every block, read from memory that no cache holds: what a tile waits for arrives late."""
