@@ -24,6 +24,8 @@
 // logit counts as -inf.  A row with logits of +inf has its mass on these, in equal shares.
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace tk {
 
 constexpr int kSelThreads = 256;
@@ -682,24 +684,25 @@ struct MoveParams {
   int per_thread;               // columns of a thread
 };
 
-template <typename V, int kSeats>
-__device__ __forceinline__ void move_columns(const MoveTensor& t, long long first, int count, const int* s_src, const int* s_dst, int n,
-                                             int max_slots) {
+// s_src, s_dst: of the n seats that change, in bytes from slot 0's record.  kExact: n is kSeats, so that nothing is asked seat by seat.
+template <typename V, int kSeats, bool kExact>
+__device__ __forceinline__ void move_columns(const MoveTensor& t, long long first, int count, const long long* s_src, const long long* s_dst,
+                                             int n, int max_slots) {
   const long long columns = t.bytes / (long long)sizeof(V), all = columns * t.keys;
 #pragma unroll 1
   for (int c = 0; c < count; ++c, first += kMoveThreads) {
     const long long at = first + threadIdx.x;
     if (at >= all) return;
     const long long key = all <= 0x7fffffffLL ? (long long)((unsigned)at / (unsigned)columns) : at / columns;
-    V* base = reinterpret_cast<V*>(t.base) + key * (max_slots - 1) * columns + at;          // column at % columns of the key's records
+    unsigned char* base = t.base + (key * (max_slots - 1) * columns + at) * (long long)sizeof(V);          // column at % columns of the key's records
     V v[kSeats];
 #pragma unroll
     for (int i = 0; i < kSeats; ++i) {
-      if (i < n) v[i] = base[(long long)s_src[i] * columns];
+      if (kExact || i < n) v[i] = *reinterpret_cast<const V*>(base + s_src[i]);
     }
 #pragma unroll
     for (int i = 0; i < kSeats; ++i) {
-      if (i < n) base[(long long)s_dst[i] * columns] = v[i];
+      if (kExact || i < n) *reinterpret_cast<V*>(base + s_dst[i]) = v[i];
     }
   }
 }
@@ -707,8 +710,11 @@ __device__ __forceinline__ void move_columns(const MoveTensor& t, long long firs
 template <int kSeats>
 __global__ void __launch_bounds__(kMoveThreads) reorder_slots_kernel(const __grid_constant__ MoveParams p) {
   pdl_trigger();
-  __shared__ int s_src[kMoveMaxSeats], s_dst[kMoveMaxSeats];
+  __shared__ long long s_src[kMoveMaxSeats], s_dst[kMoveMaxSeats];
   __shared__ int s_n;
+  int k = 0;
+  while (k + 1 < p.n_tensors && (long long)blockIdx.x >= p.t[k + 1].first_block) ++k;
+  const MoveTensor& t = p.t[k];
   pdl_wait();
   const int g = blockIdx.y;
   if (threadIdx.x < 32) {
@@ -740,8 +746,8 @@ __global__ void __launch_bounds__(kMoveThreads) reorder_slots_kernel(const __gri
       const unsigned mask = __ballot_sync(0xffffffffu, moves);
       if (moves) {
         const int at = n + __popc(mask & ((1u << lane) - 1u));
-        s_src[at] = src;
-        s_dst[at] = dst;
+        s_src[at] = src * t.bytes;
+        s_dst[at] = dst * t.bytes;
       }
       n += __popc(mask);
     }
@@ -750,15 +756,23 @@ __global__ void __launch_bounds__(kMoveThreads) reorder_slots_kernel(const __gri
   __syncthreads();
   const int n = s_n;
   if (n == 0) return;
-  int k = 0;
-  while (k + 1 < p.n_tensors && (long long)blockIdx.x >= p.t[k + 1].first_block) ++k;
-  const MoveTensor& t = p.t[k];
   const long long at = ((long long)blockIdx.x - t.first_block) * kMoveThreads * p.per_thread;
-  if (kSeats <= 32 && t.vec == 16) move_columns<uint4, (kSeats <= 32 ? kSeats : 1)>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
-  else if (t.vec == 8) move_columns<uint2, kSeats>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
-  else if (t.vec == 4) move_columns<unsigned int, kSeats>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
-  else if (t.vec == 2) move_columns<unsigned short, kSeats>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
-  else move_columns<unsigned char, kSeats>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
+  auto move = [&](auto seats, auto exact, auto type) {
+    move_columns<decltype(type), decltype(seats)::value, decltype(exact)::value>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
+  };
+  using std::integral_constant;
+  using Seats = integral_constant<int, kSeats>;
+  using Any = integral_constant<bool, false>;
+  using Exact = integral_constant<bool, true>;
+  if (t.vec == 16 && n == 1) move(integral_constant<int, 1>(), Exact(), uint4());
+  else if (t.vec == 16 && n == 2) move(integral_constant<int, 2>(), Exact(), uint4());
+  else if (t.vec == 16 && n == 3) move(integral_constant<int, 3>(), Exact(), uint4());
+  else if (t.vec == 16 && n == 4) move(integral_constant<int, 4>(), Exact(), uint4());
+  else if (kSeats <= 32 && t.vec == 16) move(integral_constant<int, (kSeats <= 32 ? kSeats : 1)>(), Any(), uint4());
+  else if (t.vec == 8) move(Seats(), Any(), uint2());
+  else if (t.vec == 4) move(Seats(), Any(), (unsigned int)0);
+  else if (t.vec == 2) move(Seats(), Any(), (unsigned short)0);
+  else move(Seats(), Any(), (unsigned char)0);
 }
 
 }  // namespace tk
