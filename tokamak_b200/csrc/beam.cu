@@ -662,8 +662,13 @@ __global__ void __launch_bounds__(64) beam_advance_kernel(AdvanceParams p) {
 // the bytes: sources that move are read, seats that change are written, nothing else is touched.
 // Before its first load a block has to know which seats change, which costs it as long as a column's loads: where there are more
 // columns than threads at a time on the device, a thread takes up to four, one after the other.  12 groups of 8 beams with 8
-// layers of 1 MB states, 313 MB to read and write: 66 us (4.7 TB/s) against 87 with a column each, 72 with two, 64 to 68
-// with eight or sixteen, which cost a call of 60 MB 14.3 us instead of 12.8.
+// layers of 1 MB states, three in ten of which change, 313 MB to read and write: 53 us (5.9 TB/s).  (With
+// twice the registers 60, 65 with two columns, 59 with eight, which cost a call of 60 MB 9.8 us instead of 9.0.)  One to
+// four seats that change have code of their own (66 us for all of them with a question for each of eight), and a kernel is held
+// to the registers that leave room for six blocks on an SM up to 8 seats, four up to 32 (8 seats: 60 us with four; 12 groups of 16:
+// 46 us with four, 62 with the two that columns of 16 bytes of all seats would leave; there more than 8 seats that change move in
+// columns of 8 bytes, more than 16 in columns of 4).  Where every seat changes that costs something: 144 us for 805 MB of 8 seats
+// instead of 128, 262 instead of 250 for 1.6 GB of 16, 331 instead of 255 of 32.
 constexpr int kMoveThreads = 256;
 constexpr int kMoveColumns = 4;
 constexpr int kMoveMaxTensors = 24;
@@ -708,7 +713,7 @@ __device__ __forceinline__ void move_columns(const MoveTensor& t, long long firs
 }
 
 template <int kSeats>
-__global__ void __launch_bounds__(kMoveThreads) reorder_slots_kernel(const __grid_constant__ MoveParams p) {
+__global__ void __launch_bounds__(kMoveThreads, kSeats <= 8 ? 6 : kSeats <= 32 ? 4 : 2) reorder_slots_kernel(const __grid_constant__ MoveParams p) {
   pdl_trigger();
   __shared__ long long s_src[kMoveMaxSeats], s_dst[kMoveMaxSeats];
   __shared__ int s_n;
@@ -757,22 +762,24 @@ __global__ void __launch_bounds__(kMoveThreads) reorder_slots_kernel(const __gri
   const int n = s_n;
   if (n == 0) return;
   const long long at = ((long long)blockIdx.x - t.first_block) * kMoveThreads * p.per_thread;
+  // columns of the tensor's width, or of a part of it where so many seats change that a thread's registers would not hold them
   auto move = [&](auto seats, auto exact, auto type) {
-    move_columns<decltype(type), decltype(seats)::value, decltype(exact)::value>(t, at, p.per_thread, s_src, s_dst, n, p.max_slots);
+    const int parts = t.vec / (int)sizeof(type);
+    move_columns<decltype(type), decltype(seats)::value, decltype(exact)::value>(t, at * parts, p.per_thread * parts, s_src, s_dst, n, p.max_slots);
   };
   using std::integral_constant;
-  using Seats = integral_constant<int, kSeats>;
   using Any = integral_constant<bool, false>;
   using Exact = integral_constant<bool, true>;
+  constexpr int kEight = kSeats < 8 ? kSeats : 8, kSixteen = kSeats < 16 ? kSeats : 16;
   if (t.vec == 16 && n == 1) move(integral_constant<int, 1>(), Exact(), uint4());
   else if (t.vec == 16 && n == 2) move(integral_constant<int, 2>(), Exact(), uint4());
   else if (t.vec == 16 && n == 3) move(integral_constant<int, 3>(), Exact(), uint4());
   else if (t.vec == 16 && n == 4) move(integral_constant<int, 4>(), Exact(), uint4());
-  else if (kSeats <= 32 && t.vec == 16) move(integral_constant<int, (kSeats <= 32 ? kSeats : 1)>(), Any(), uint4());
-  else if (t.vec == 8) move(Seats(), Any(), uint2());
-  else if (t.vec == 4) move(Seats(), Any(), (unsigned int)0);
-  else if (t.vec == 2) move(Seats(), Any(), (unsigned short)0);
-  else move(Seats(), Any(), (unsigned char)0);
+  else if (t.vec == 16 && n <= kEight) move(integral_constant<int, kEight>(), Any(), uint4());
+  else if (t.vec >= 8 && n <= kSixteen) move(integral_constant<int, kSixteen>(), Any(), uint2());
+  else if (t.vec >= 4) move(integral_constant<int, kSeats>(), Any(), (unsigned int)0);
+  else if (t.vec == 2) move(integral_constant<int, kSeats>(), Any(), (unsigned short)0);
+  else move(integral_constant<int, kSeats>(), Any(), (unsigned char)0);
 }
 
 }  // namespace tk
@@ -843,8 +850,6 @@ TK_API int tk_reorder_slots(const long long* tensors, int n_tensors, const int* 
     t.bytes = bytes;
     t.keys = (int)keys;
     t.vec = 16;
-    // 64 seats of 16 bytes would not fit a thread's registers
-    if (seats > 32) t.vec = 8;
     while (((unsigned long long)base | (unsigned long long)bytes) % (unsigned long long)t.vec) t.vec /= 2;
     columns += t.bytes / t.vec * t.keys;
   }
