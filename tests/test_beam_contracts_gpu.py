@@ -1,0 +1,42 @@
+"""What the operators of a search over beams say of themselves, held to the last place that they promise."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from test_beam_kernels_gpu import BF16_HALF, DEV, F32_HALF, Shared, err_word, i32
+from tokamak_b200.csrc import ops
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ attention
+
+def check_one_rounding(c):
+    """Of a bfloat16 result only its own rounding may be seen: a probability is two bfloat16, so what is left of its rounding is the
+    second's, a half step of a half step; scores and sums are floats."""
+    want, weight, size = c.oracle()
+    score = (c.d + 4) * F32_HALF * size + 2.0 ** -22 + (1e-6 * c.softcap if c.softcap else 0.0)
+    keys = int(c.positions.max()) + 1
+    tol = (2 * score + keys ** 0.5 * F32_HALF * 4 + BF16_HALF * BF16_HALF) * weight
+    off = (c.out.cpu().double() - want).abs()
+    beyond = off - (tol + BF16_HALF * (want.abs() + tol))
+    assert beyond.max() <= 0, f"{int((beyond > 0).sum())} of {beyond.numel()} elements are off by more than their rounding"
+    assert c.err.tolist() == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("form", [
+    dict(members=[4], prefixes=[700], own=1),                                         # shared positions, groups of lanes in turns
+    dict(members=[40, 33], prefixes=[300, 200], own=1, hq=8),                         # two tiles of query rows
+    dict(members=[6], prefixes=[130], own=90, history=True, common=80),               # a common past
+    dict(members=[3], prefixes=[0], own=150, hq=8),                                   # own positions alone
+    dict(members=[5], prefixes=[40], own=200, history=True),                          # own positions of several writers
+    dict(members=[2], prefixes=[70], own=600),                                        # cut into parts
+    dict(members=[4], prefixes=[500], own=60, history=True, window=256, softcap=30.0, sinks=True)])
+def test_shared_attention_is_off_by_its_own_rounding_only(form, d):
+    c = Shared(**form, d=d, dtype=torch.bfloat16, seed=31).device()
+    c.call()
+    check_one_rounding(c)

@@ -17,15 +17,17 @@
 //                straight from its page layout.  (A product costs the thread that issues it 77 clocks whatever its N up to 128:
 //                one thread for both groups needed 1,820 clocks a tile.)
 //   warps 2..5, 6..9   softmax, two groups with an output accumulator each, thread i owns row i of its tile: scores with
-//                tcgen05.ld, mask, running reference and sum in float32, probabilities as bfloat16 pairs over the scores.  The
-//                output is rescaled in tensor memory only when a row's maximum grew by more than 2^8 since its reference
-//                was set.  With more than 128 rows the two groups have a tile of rows each and every key tile; with fewer they
+//                tcgen05.ld, mask, running reference and sum in float32, probabilities over the scores.  The output is rescaled
+//                in tensor memory only when a row's maximum grew by more than 2^8 since its reference was set.  With more than 128 rows the two groups have a tile of rows each and every key tile; with fewer they
 //                take turns at the key tiles, so that the softmax of two of them is under way at a time.
+// A probability is two bfloat16 here, its rounded value and what the rounding left, and P V a product of either, in both kernels:
+// the sum that divides the output has the probabilities as floats, so that one rounding of each would stay in the result (2.1e-3 of it
+// where the result's own is 1.66e-3).  It costs 4 to 10 %: 65 us instead of 61 for 16 groups of 4, 126 instead of 114 for 4 of 16.
 // Bound: the keys' bytes.  A tile of 64 keys of 128 elements is 32 KB, 0.74 us of an SM's share of the memory bandwidth, against
-// 0.38 us of tensor time; one softmax group needs 1.2 us for it, the two together 0.6.  Measured within a long run of tiles: 0.8
-// us each, 5.9 TB/s in all.  A call of 4 groups of 16 rows, 32 query heads over 8 of 128, 32,768 shared and 1,024 further positions
-// (456 MB) takes 110 us, one of 16 groups of 4 over up to 4,093 + 129 (216 MB) 60: the plan is 3 to 6 us of that, the first
-// tile's way 4, a change of group 3, the rows' own positions and the parts 10 behind it all.
+// 0.5 us of tensor time; a softmax group needs more than a microsecond for it, the two together half of that.  A call of 4 groups of
+// 16 rows, 32 query heads over 8 of 128, 32,768 shared and 1,024 further positions (456 MB) takes 126 us, one of 16 groups of 4 over up
+// to 4,093 + 129 (216 MB) 65: the plan is 3 to 6 us of that, the first tile's way 4, a change of group 3, the rows' own positions and the
+// parts 10 behind it all.
 //
 // Rows of V that no row may see (behind the prefix in its last page, in front of a window) are zeroed in shared memory
 // before they are used: their probabilities are zero, and what lies there may be anything.
@@ -221,6 +223,11 @@ __device__ __forceinline__ float sp_rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
+}
+
+// What is left of a and b behind their roundings in `hi`, as bfloat16.
+__device__ __forceinline__ uint32_t rest_bf16(float a, float b, uint32_t hi) {
+  return pack_bf16(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
 }
 
 template <int D>
@@ -532,8 +539,10 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
               const uint64_t db0 = desc_v + (uint64_t)(st_v * (KV_BYTES >> 4));
 #pragma unroll
               for (int kk = 0; kk < kSpBN / 16; ++kk) {
-                umma_bf16_ts(tmem_o, tmem_s + (uint32_t)(bf * kSpBN + 8 * kk), db0 + (uint64_t)(kk * ((16 * 128) >> 4)), idesc_o,
-                             (n > 1 || kk > 0) ? 1u : 0u);
+                const uint64_t db = db0 + (uint64_t)(kk * ((16 * 128) >> 4));
+                const uint32_t a = tmem_s + (uint32_t)(bf * kSpBN + (kk / 2) * 32 + (kk % 2) * 8);
+                umma_bf16_ts(tmem_o, a, db, idesc_o, (n > 1 || kk > 0) ? 1u : 0u);
+                umma_bf16_ts(tmem_o, a + 16u, db, idesc_o, 1u);
               }
               umma_commit(pv_done(t, bf));
               if (n == n_mine) umma_commit(o_full(t));
@@ -668,16 +677,20 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
             const float m_use = (m_ref == -INFINITY) ? 0.0f : m_ref;
             float2 psum = make_float2(0.0f, 0.0f);
             const float2 scale2 = make_float2(eff_scale, eff_scale), shift2 = make_float2(-m_use, -m_use);
-            uint32_t packed[kSpBN / 2];
 #pragma unroll
-            for (int c = 0; c < kSpBN; c += 2) {
-              const float2 y = fma2(make_float2(sv[c], sv[c + 1]), scale2, shift2);
-              const float2 e = make_float2(sp_ex2(y.x), sp_ex2(y.y));
-              psum = add2(psum, e);
-              packed[c / 2] = pack_bf16(e.x, e.y);
+            for (int half = 0; half < kSpBN; half += 32) {
+              uint32_t packed[32];         // 32 keys' rounded probabilities, then what the rounding left of each
+#pragma unroll
+              for (int c = 0; c < 32; c += 2) {
+                const float2 y = fma2(make_float2(sv[half + c], sv[half + c + 1]), scale2, shift2);
+                const float2 e = make_float2(sp_ex2(y.x), sp_ex2(y.y));
+                psum = add2(psum, e);
+                packed[c / 2] = pack_bf16(e.x, e.y);
+                packed[16 + c / 2] = rest_bf16(e.x, e.y, packed[c / 2]);
+              }
+              tmem_st32(tmem_s + (uint32_t)(bf * kSpBN + half), packed);
             }
             l_sum += psum.x + psum.y;
-            tmem_st32(tmem_s + (uint32_t)(bf * kSpBN), packed);
             tmem_wait_st();
             tc_fence_before();
           }
@@ -987,6 +1000,8 @@ shared_own_kernel(const __grid_constant__ SharedParams p, const __grid_constant_
       }
       const uint32_t pa0 = pack_bf16(s[0][0], s[0][1]), pa1 = pack_bf16(s[0][2], s[0][3]);
       const uint32_t pa2 = pack_bf16(s[1][0], s[1][1]), pa3 = pack_bf16(s[1][2], s[1][3]);
+      const uint32_t pr0 = rest_bf16(s[0][0], s[0][1], pa0), pr1 = rest_bf16(s[0][2], s[0][3], pa1);
+      const uint32_t pr2 = rest_bf16(s[1][0], s[1][1], pa2), pr3 = rest_bf16(s[1][2], s[1][3], pa3);
 #pragma unroll
       for (int c = 0; c < D / 8; c += 2) {
         const int r = (((lane >> 3) & 1) << 3) + (lane & 7);
@@ -995,6 +1010,8 @@ shared_own_kernel(const __grid_constant__ SharedParams p, const __grid_constant_
         ldmatrix_x4_trans(vbase + swizzled_offset(r, chunk, CH), b0, b1, b2, b3);
         mma_bf16_16816(o[c], pa0, pa1, pa2, pa3, b0, b1);
         mma_bf16_16816(o[c + 1], pa0, pa1, pa2, pa3, b2, b3);
+        mma_bf16_16816(o[c], pr0, pr1, pr2, pr3, b0, b1);
+        mma_bf16_16816(o[c + 1], pr0, pr1, pr2, pr3, b2, b3);
       }
       __syncwarp();
     }
