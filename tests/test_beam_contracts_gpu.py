@@ -40,3 +40,26 @@ def test_shared_attention_is_off_by_its_own_rounding_only(form, d):
     c = Shared(**form, d=d, dtype=torch.bfloat16, seed=31).device()
     c.call()
     check_one_rounding(c)
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 32)])
+@pytest.mark.parametrize("history", [False, True])
+@pytest.mark.parametrize("window", [None, 50])
+def test_a_row_with_a_position_that_is_none_sees_nothing(window, history, dtype, d):
+    """Not the shared positions either; the other members of its group are what they are without it."""
+    c = Shared([3, 2], [140, 50], 20, d=d, dtype=dtype, history=history, window=window, seed=12).device()
+    c.call()
+    c.check()
+    whole = c.out.clone()
+    place = c.table.shape[1] * c.page                    # the first position that the block table has no place for
+    for bad in (place, 10 ** 6, -1, -10 ** 6):
+        positions = c.positions.copy()
+        positions[[1, 4]] = bad
+        c.out.fill_(float("nan"))
+        c.err.zero_()
+        ops.attention_shared(c.dq, c.out, c.dk, c.dv_, c.shared(), i32(positions), *c.args[1:], **c.kw)
+        assert c.err.tolist()[0] == 3
+        assert bool((c.out[[1, 4]] == 0).all()), bad
+        # (parts may be cut elsewhere without a common past: floats are added in another order)
+        half = BF16_HALF if dtype == torch.bfloat16 else F32_HALF
+        torch.testing.assert_close(c.out[[0, 2, 3]].float(), whole[[0, 2, 3]].float(), rtol=2 * half, atol=2.0 ** -12)

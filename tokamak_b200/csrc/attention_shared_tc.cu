@@ -578,7 +578,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         const bool active = quarter * 32 < n_rows;         // warps without rows keep the barriers' count and do nothing else
         const int tok = x.row0 + (both ? t * mpt : 0) + row / per, head = x.hkv * per + row % per;
         RowSpan sp = {0x7fffffff, 0};                      // a lane without a row masks nothing: nobody reads what comes of it
-        if (row < n_rows) { sp.pos = p.positions[tok]; sp.lo = first_visible(sp.pos, p.window, 0); }
+        if (row < n_rows) sp = row_span(p, tok);
         const int j0 = both ? 0 : t, step = both ? 1 : 2;
         const int n_mine = both ? x.n_tiles : (x.n_tiles - t + 1) / 2;
         float m_ref = -INFINITY, l_sum = 0.0f;
