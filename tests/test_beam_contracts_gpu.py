@@ -63,3 +63,50 @@ def test_a_row_with_a_position_that_is_none_sees_nothing(window, history, dtype,
         # (parts may be cut elsewhere without a common past: floats are added in another order)
         half = BF16_HALF if dtype == torch.bfloat16 else F32_HALF
         torch.testing.assert_close(c.out[[0, 2, 3]].float(), whole[[0, 2, 3]].float(), rtol=2 * half, atol=2.0 ** -12)
+
+
+# ------------------------------------------------------------------------------------------------ selection
+
+def ranked(x: np.ndarray, scores: np.ndarray, k: int):
+    """``(keys, parents, tokens)`` as ``ops.beam_select`` describes them, in 64 bits: by key, then the lower beam, then the larger
+    logit, then the lower token.  Finite logits and scores."""
+    groups, beams = scores.shape
+    vocab = x.shape[1]
+    wide = x.astype(np.float64)
+    d = wide - wide.max(axis=1, keepdims=True)
+    keys = scores.astype(np.float64).reshape(-1, 1) + (d - np.log(np.exp(d).sum(axis=1, keepdims=True)))
+    beam, token = np.divmod(np.arange(beams * vocab), vocab)
+    out = []
+    for g in range(groups):
+        rows = slice(g * beams, (g + 1) * beams)
+        order = np.lexsort((token, -wide[rows].reshape(-1), beam, -keys[rows].reshape(-1)))[:k]
+        out.append((keys[rows].reshape(-1)[order], beam[order], token[order]))
+    return tuple(np.stack(a) for a in zip(*out))
+
+
+@pytest.mark.parametrize("beams,vocab,k", [(2, 2, 4), (3, 50, 40), (8, 9001, 64), (64, 4099, 256), (4, 50001, 16)])
+def test_equal_scores_of_beams_whose_logits_differ_by_a_constant(beams, vocab, k):
+    """Rows of whole numbers that differ by a whole number have the same keys to the last bit: the lower beam comes first, whatever
+    its logits are."""
+    rng = np.random.default_rng(vocab)
+    base = rng.integers(-9, 6, (2, 1, vocab))
+    x = (base + rng.permutation(np.arange(beams) * 5 - beams)[None, :, None]).reshape(2 * beams, vocab).astype(np.float32)
+    s = np.full((2, beams), -3.0, dtype=np.float32)
+    got = ops.beam_select(torch.from_numpy(x).to(DEV), torch.from_numpy(s).to(DEV), k)
+    keys, parents, tokens = ranked(x, s, k)
+    assert (keys[:, 1:] == keys[:, :-1]).any()
+    np.testing.assert_array_equal(got[1].cpu().numpy(), parents)
+    np.testing.assert_array_equal(got[2].cpu().numpy(), tokens)
+
+
+def test_equal_scores_of_one_beam_go_by_the_logit():
+    """Logits so small beside the row's largest that their keys are the same in 64 bits."""
+    x = np.zeros((4, 40), dtype=np.float32)
+    x[:, 7] = 12.0
+    x[:, 8:40] = np.float32(1e-30) * np.arange(1, 33, dtype=np.float32)
+    s = np.full((1, 4), -1.0, dtype=np.float32)
+    got = ops.beam_select(torch.from_numpy(x).to(DEV), torch.from_numpy(s).to(DEV), 60)
+    keys, parents, tokens = ranked(x, s, 60)
+    assert tokens[0, 4:8].tolist() == [39, 38, 37, 36] and parents[0, 4:36].tolist() == [0] * 32
+    np.testing.assert_array_equal(got[1].cpu().numpy(), parents)
+    np.testing.assert_array_equal(got[2].cpu().numpy(), tokens)

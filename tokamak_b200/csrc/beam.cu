@@ -3,8 +3,8 @@
 // Selection.  Beam w of a group has a score s_w (the sum of its tokens' log probabilities) and a row of logits x_w; its
 // continuation by token v has the key
 //     key(w, v) = s_w + ((x_wv - M_w) - log sum_u exp(x_wu - M_w)),      M_w any reference of the row,
-// and the K largest keys of a group's W * V are wanted in order; equal keys of one beam by the larger logit, others by the
-// lowest w * V + v.  Keys of neighbouring ranks differ by less than a float's last place often enough to change what a
+// and the K largest keys of a group's W * V are wanted in order; equal keys: the lower beam, of one beam the larger logit, then
+// the lower token.  Keys of neighbouring ranks differ by less than a float's last place often enough to change what a
 // search does, so sums and keys are 64-bit: the exponentials are floats (an error of some 1e-7 each that falls away in the
 // sum, where the largest terms, those of the candidates, are put right in 64 bits), added four at a time as floats and then as
 // doubles.
@@ -38,6 +38,7 @@ constexpr int kSelBuffer = 2048;                               // elements set a
 constexpr int kJoinThreads = 512;                              // and so many are ranked by comparing each with each
 constexpr int kSelMaxK = 256;
 constexpr int kSelMaxBeams = 64;
+constexpr int kSelTokenBits = 26;                              // of a token in what ranks behind a key
 constexpr int kSelMaxEntries = 16384;                          // beams * segments * K that a joining block takes
 constexpr float kSelRaise = 60.0f;                             // exponents above the reference that the sums hold
 
@@ -460,11 +461,14 @@ beam_join_kernel(SelectParams p) {
   // Keys as floats, rounded down, are in the keys' order but for what they round away, and half the bits to look at.
   auto as_float = [&](unsigned long long key) { return key == 0ull ? 0u : ordered_f32(__double2float_rd(from_ordered_f64(key))); };
   auto from_float = [&](unsigned int t32) { return t32 <= ordered_f32(-INFINITY) ? 1ull : ordered_f64((double)from_ordered_f32(t32)); };
-  // what comes after the key: the logit where it decides, then the place
+  // what comes after the key: the beam, the logit where there is one, the token (logits of different beams cannot be compared)
+  constexpr unsigned int kTokens = 1u << kSelTokenBits;
+  static_assert(kSelMaxBeams == 1 << (64 - 32 - kSelTokenBits), "a beam, a logit and a token in 64 bits");
   auto second_of = [&](int i, unsigned long long key, unsigned long long elem) {
-    const unsigned int place = (unsigned int)(i / per_row) * (unsigned int)p.vocab + (0xffffffffu - (unsigned int)elem);
+    const unsigned int token = 0xffffffffu - (unsigned int)elem;
     const unsigned int logit = key == ordered_f64(-INFINITY) ? 0u : (unsigned int)(elem >> 32);
-    return ((unsigned long long)logit << 32) | (0xffffffffu - place);
+    return ((unsigned long long)(kSelMaxBeams - 1 - i / per_row) << (32 + kSelTokenBits)) |
+           ((unsigned long long)logit << kSelTokenBits) | (kTokens - 1u - token);
   };
   const unsigned long long my_key = my_elem == 0ull ? 0ull : key_of((int)threadIdx.x / per_row, my_elem);
   int m = 0;
@@ -572,10 +576,9 @@ beam_join_kernel(SelectParams p) {
     const int rank = s_rank[threadIdx.x];
     if (rank < p.k) {
       const size_t at = (size_t)group * p.k + rank;
-      const unsigned int place = 0xffffffffu - (unsigned int)b;
       p.out_scores[at] = (float)from_ordered_f64(a);
-      p.out_parents[at] = (int)(place / (unsigned int)p.vocab);
-      p.out_tokens[at] = (int)(place % (unsigned int)p.vocab);
+      p.out_parents[at] = kSelMaxBeams - 1 - (int)(b >> (32 + kSelTokenBits));
+      p.out_tokens[at] = (int)(kTokens - 1u - ((unsigned int)b & (kTokens - 1u)));
     }
   }
 }
@@ -790,7 +793,7 @@ TK_API int tk_beam_select(const float* logits, long long ld, const float* scores
                           cudaStream_t stream) {
   if (groups <= 0) return 0;
   if (beams < 1 || beams > tk::kSelMaxBeams || k < 1 || k > tk::kSelMaxK || vocab < 1 || segments < 1 || ld < vocab ||
-      (long long)beams * segments * k > tk::kSelMaxEntries || (long long)beams * vocab > 0x7fffffffLL ||
+      (long long)beams * segments * k > tk::kSelMaxEntries || vocab > 1 << tk::kSelTokenBits ||
       (long long)groups * beams > 65535 || (long long)k > (long long)beams * vocab) {
     return (int)cudaErrorInvalidValue;
   }
