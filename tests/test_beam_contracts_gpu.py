@@ -110,3 +110,34 @@ def test_equal_scores_of_one_beam_go_by_the_logit():
     assert tokens[0, 4:8].tolist() == [39, 38, 37, 36] and parents[0, 4:36].tolist() == [0] * 32
     np.testing.assert_array_equal(got[1].cpu().numpy(), parents)
     np.testing.assert_array_equal(got[2].cpu().numpy(), tokens)
+
+
+def nearly_equal(kind, beams, vocab, seed):
+    """Rows of logits, and scores with which the best continuations of all beams have keys within a score's last place."""
+    rng = np.random.default_rng(seed)
+    x = (rng.standard_normal((beams, vocab)) * 2.5).astype(np.float32)
+    if kind == "low_start":                    # what a row begins with is far below the rest
+        x[:, :vocab // 3] -= np.float32(20.0) + np.arange(beams, dtype=np.float32)[:, None] * np.float32(0.37)
+    elif kind == "high":                       # a few tokens well above the rest, anywhere
+        x[np.arange(beams)[:, None], rng.integers(0, vocab, (beams, 24))] += (rng.random((beams, 24)) * 9.0).astype(np.float32)
+    elif kind == "flat":                       # many tokens that weigh alike, rows at different heights
+        x = x * np.float32(0.2) + np.arange(beams, dtype=np.float32)[:, None] * np.float32(1.7)
+    wide = x.astype(np.float64)
+    top = wide.max(axis=1)
+    logp = -np.log(np.exp(wide - top[:, None]).sum(axis=1))
+    return x, (logp[0] - logp).astype(np.float32)[None, :]
+
+
+@pytest.mark.parametrize("kind,beams,vocab,seed", [("normal", 64, 20011, 1), ("normal", 24, 151936, 2), ("low_start", 64, 20011, 3),
+                                                   ("low_start", 24, 100003, 4), ("high", 64, 50001, 5), ("flat", 64, 20011, 6)])
+def test_scores_that_nearly_are_equal_come_in_their_order(kind, beams, vocab, seed):
+    x, s = nearly_equal(kind, beams, vocab, seed)
+    keys, parents, tokens = ranked(x, s, beams)
+    gaps = -np.diff(keys[0])
+    # a row's logarithm is off by up to 1.5e-13 for the series of its exponentials and, sums of some hundred additions a thread and a tree
+    # over the threads, by 100 * 2^-53 = 1.2e-14 for each side's sums; a key near 10 by 2^-50: two rows by 3.5e-13 in all
+    assert gaps.min() > 4e-13 and np.median(gaps) < 2e-8
+    for k in (beams, 1, 5, beams // 2):              # the last that is wanted, and the one behind it, are as close
+        got = ops.beam_select(torch.from_numpy(x).to(DEV), torch.from_numpy(s).to(DEV), k)
+        np.testing.assert_array_equal(got[1].cpu().numpy(), parents[:, :k])
+        np.testing.assert_array_equal(got[2].cpu().numpy(), tokens[:, :k])

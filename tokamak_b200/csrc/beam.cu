@@ -5,9 +5,12 @@
 //     key(w, v) = s_w + ((x_wv - M_w) - log sum_u exp(x_wu - M_w)),      M_w any reference of the row,
 // and the K largest keys of a group's W * V are wanted in order; equal keys: the lower beam, of one beam the larger logit, then
 // the lower token.  Keys of neighbouring ranks differ by less than a float's last place often enough to change what a
-// search does, so sums and keys are 64-bit: the exponentials are floats (an error of some 1e-7 each that falls away in the
-// sum, where the largest terms, those of the candidates, are put right in 64 bits), added four at a time as floats and then as
-// doubles.
+// search does, so sums and keys are 64-bit.  The exponentials are floats, added four at a time as floats and then as doubles, and the
+// largest, those of the candidates, are put right in 64 bits: a row's logarithm is off by some 1e-8 to 1e-7, each row's by its own,
+// and two rows' by no more than order_bound() says.  Where continuations of different beams are closer than that and it matters, the
+// joining kernel forms the sums of their rows again, with every exponential in 64 bits, and ranks once more: in one call of
+// forty of 32 groups of 16 beams, which then takes 60 us more.  (With all exponentials in 64 bits each of these calls takes 103 us
+// instead of 56.)
 //
 // One pass over the logits.  Within a row the order of the keys is that of the logits, so the K best of a row's segment can
 // be kept without knowing the row's sum: a block streams its segment in tiles, holds a threshold with at least K elements
@@ -16,7 +19,7 @@
 // group: it adds the segments' sums up in their order, makes the keys of the elements set aside and ranks them.  Two kernels and
 // no counter: calls on two streams, or two captured graphs, share nothing.
 //
-// Bound by the logits' bytes where there are many: 205 MB (512 rows of 100,003) in 54 us, 3.8 TB/s; what is left are the
+// Bound by the logits' bytes where there are many: 205 MB (512 rows of 100,003) in 56 us, 3.7 TB/s; what is left are the
 // instructions beside the loads, an exponential and a comparison a logit (44 us without either).  Few rows are bound by
 // latency: 10 us for one row of 151,936, 14 for 32.
 //
@@ -40,7 +43,7 @@ constexpr int kSelMaxK = 256;
 constexpr int kSelMaxBeams = 64;
 constexpr int kSelTokenBits = 26;                              // of a token in what ranks behind a key
 constexpr int kSelMaxEntries = 16384;                          // beams * segments * K that a joining block takes
-constexpr float kSelRaise = 60.0f;                             // exponents above the reference that the sums hold
+constexpr float kSelRaise = 12.0f;                             // exponents above the reference that the sums hold
 
 struct SelectParams {
   const float* logits;          // [groups * beams, vocab], row stride ld
@@ -195,6 +198,50 @@ __device__ __forceinline__ float2 terms_f32(float x, float y, float ref) {
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(d.x));
   asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(d.y));
   return d;
+}
+
+// How far apart the logarithms of two rows' sums may be from what they are by the float exponentials.  A term e^d is off by 2^-24 |d|
+// each for the roundings of d and of d log2(e), 1.4e-8 |d| for the constant's, 2^-22 for the power of two and 2^-23 for two additions,
+// relative to itself.  Weighed by the terms themselves, |d| is no more than kSelRaise where d > 0, and, since the reference is a term,
+// no more than ln(vocab) where d < 0; both kinds together no more than the larger of the two and 1 / e.
+__device__ __forceinline__ double order_bound(int vocab) {
+  return 2.0 * (1.34e-7 * ((double)fmaxf(kSelRaise, logf((float)vocab)) + 0.4) + 3.7e-7);
+}
+
+// Exponentials in 64 bits, added to one of two sums in turn, of d = x - ref in (-87, 87): 2^(k / 16) from a table, times the series of e^r up to r^5 / 120,
+// r = d - k ln(2) / 16 (table-driven, after P. T. P. Tang, 1989).  |r| <= ln(2) / 32, so the terms left out are less than 1.5e-13
+// of it.
+__constant__ double kPowers[16] = {           // 2^(j / 16)
+    0x1.0000000000000p+0, 0x1.0b5586cf9890fp+0, 0x1.172b83c7d517bp+0, 0x1.2387a6e756238p+0,
+    0x1.306fe0a31b715p+0, 0x1.3dea64c123422p+0, 0x1.4bfdad5362a27p+0, 0x1.5ab07dd485429p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.7a11473eb0187p+0, 0x1.8ace5422aa0dbp+0, 0x1.9c49182a3f090p+0,
+    0x1.ae89f995ad3adp+0, 0x1.c199bdd85529cp+0, 0x1.d5818dcfba487p+0, 0x1.ea4afa2a490dap+0};
+template <int N>
+__device__ __forceinline__ void add_terms(double (&sum)[2], const float* x, float ref, double ref64, const double* powers) {
+  const double whole = 6755399441055744.0;             // 1.5 * 2^52: what is added to it is rounded to a whole number
+  double r[N], scaled[N], e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const double d = (double)x[i] - ref64, shifted = fma(d, 0x1.71547652b82fep+4, whole);
+    const int k = __double2loint(shifted);
+    r[i] = fma(shifted - whole, -0x1.62e42fefa39efp-5, d);
+    const double t = powers[k & 15];
+    scaled[i] = __hiloint2double(__double2hiint(t) + ((k & ~15) << 16), __double2loint(t));
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = fma(r[i], 1.0 / 120.0, 1.0 / 24.0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = fma(r[i], e[i], 1.0 / 6.0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = fma(r[i], e[i], 0.5);
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = fma(r[i], e[i], 1.0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = fma(r[i], e[i], 1.0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (x[i] - ref > -87.0f) sum[i & 1] = fma(scaled[i], e[i], sum[i & 1]);          // e^-87 is nothing beside the reference's own term
+  }
 }
 
 // kPerSm: blocks on an SM at a time.  Four leave a thread 64 registers, and it keeps some of its values in memory; where there are
@@ -407,23 +454,49 @@ beam_segments_kernel(SelectParams p) {
   }
 }
 
+// A row's sum with every exponential in 64 bits; `parts` is for a value of each of the block's warps.  28 us for a row of 100,003.
+// (Shared out over a cluster of eight blocks a group 9 us, but then every call takes 2 us more.)
+__device__ __noinline__ double sum_again(const float* x, int vocab, double ref, const double* powers, double* parts) {
+  constexpr int AHEAD = 16;
+  double two[2] = {0.0, 0.0};
+  for (int i0 = threadIdx.x; i0 < vocab; i0 += AHEAD * kJoinThreads) {
+    float v[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) v[j] = i0 + j * kJoinThreads < vocab ? fmaxf(x[i0 + j * kJoinThreads], -INFINITY) : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < AHEAD; j += 4) add_terms<4>(two, v + j, (float)ref, ref, powers);
+  }
+  double sum = two[0] + two[1];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) sum += parts[i];
+  return sum;
+}
+
 // One block per group: the sums of its rows, the keys of the elements set aside, the K best of them in order.  A segment's elements
 // come best first, so where there are more segments than K only those whose first is among the K best firsts matter.
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(kJoinThreads, 2)
 beam_join_kernel(SelectParams p) {
   pdl_trigger();
   extern __shared__ unsigned long long s_key[];                // [beams * segments * K] keys in their order
   __shared__ double s_ref[kSelMaxBeams], s_log[kSelMaxBeams];
   __shared__ unsigned long long s_best[kJoinThreads];
   __shared__ unsigned long long s_second[kJoinThreads];
+  __shared__ unsigned long long s_top[kSelMaxK], s_top_second[kSelMaxK], s_doubt;
+  __shared__ double s_powers[16], s_part[kJoinThreads / 32];
   __shared__ int s_count, s_rank[kJoinThreads];
   const int group = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const size_t row0 = (size_t)group * p.beams;
   const int per_row = p.segments * p.k;
   const int n = p.beams * per_row, lists = p.beams * p.segments;
-  if (threadIdx.x == 0) s_count = 0;
-  s_rank[threadIdx.x] = 0;
+  if (threadIdx.x == 0) s_doubt = 0ull;
+  if (threadIdx.x < 16) s_powers[threadIdx.x] = kPowers[threadIdx.x];
   pdl_wait();
   const unsigned long long* elems = p.seg_key + row0 * per_row;
   const bool one_each = n <= kJoinThreads;                     // a thread has one element: it stays in a register
@@ -470,116 +543,164 @@ beam_join_kernel(SelectParams p) {
     return ((unsigned long long)(kSelMaxBeams - 1 - i / per_row) << (32 + kSelTokenBits)) |
            ((unsigned long long)logit << kSelTokenBits) | (kTokens - 1u - token);
   };
-  const unsigned long long my_key = my_elem == 0ull ? 0ull : key_of((int)threadIdx.x / per_row, my_elem);
-  int m = 0;
-  if (!one_each) {
-    unsigned long long t = 1ull;                                   // everything there is
-    if (lists > p.k) {
-      for (int i = threadIdx.x; i < lists; i += kJoinThreads) s_key[i * p.k] = any_key(i * p.k);
-      __syncthreads();
-      if (lists <= kJoinThreads) {
-        const unsigned long long key = (int)threadIdx.x < lists ? s_key[threadIdx.x * p.k] : 0ull;
-        t = from_float(block_threshold_of<unsigned int>(p.k, p.k, key != 0ull, as_float(key)));
-      } else {
-        t = from_float(block_threshold<kJoinThreads, unsigned int>(p.k, p.k + p.k / 4, [&](unsigned int trial) {
-          int c = 0;
-          for (int i = threadIdx.x; i < lists; i += kJoinThreads) c += as_float(s_key[i * p.k]) >= trial ? 1 : 0;
-          return c;
-        }));
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < n; i += kJoinThreads) {
-        const int list = i / p.k, first = list * p.k;
-        if (i != first) s_key[i] = s_key[first] >= t ? any_key(i) : 0ull;
-      }
-    } else {
-      for (int i = threadIdx.x; i < n; i += kJoinThreads) s_key[i] = any_key(i);
-    }
+  // twice where the first time leaves it in doubt which of two beams' continuations is ranked higher
+  for (int pass = 0;; ++pass) {
+    s_rank[threadIdx.x] = 0;
+    if (threadIdx.x == 0) s_count = 0;
     __syncthreads();
-    auto gather = [&](unsigned long long t, unsigned long long t2) {
+    const unsigned long long my_key = my_elem == 0ull ? 0ull : key_of((int)threadIdx.x / per_row, my_elem);
+    int m = 0;
+    if (!one_each) {
+      unsigned long long t = 1ull;                                   // everything there is
+      if (lists > p.k) {
+        for (int i = threadIdx.x; i < lists; i += kJoinThreads) s_key[i * p.k] = any_key(i * p.k);
+        __syncthreads();
+        if (lists <= kJoinThreads) {
+          const unsigned long long key = (int)threadIdx.x < lists ? s_key[threadIdx.x * p.k] : 0ull;
+          t = from_float(block_threshold_of<unsigned int>(p.k, p.k, key != 0ull, as_float(key)));
+        } else {
+          t = from_float(block_threshold<kJoinThreads, unsigned int>(p.k, p.k + p.k / 4, [&](unsigned int trial) {
+            int c = 0;
+            for (int i = threadIdx.x; i < lists; i += kJoinThreads) c += as_float(s_key[i * p.k]) >= trial ? 1 : 0;
+            return c;
+          }));
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += kJoinThreads) {
+          const int list = i / p.k, first = list * p.k;
+          if (i != first) s_key[i] = s_key[first] >= t ? any_key(i) : 0ull;
+        }
+      } else {
+        for (int i = threadIdx.x; i < n; i += kJoinThreads) s_key[i] = any_key(i);
+      }
+      __syncthreads();
+      auto gather = [&](unsigned long long t, unsigned long long t2) {
+        __syncthreads();
+        if (threadIdx.x == 0) s_count = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += kJoinThreads) {
+          const unsigned long long key = s_key[i];
+          if (key < t) continue;
+          const unsigned long long second = second_of(i, s_key[i], __ldcg(elems + i));
+          if (key > t || second >= t2) {
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kJoinThreads) { s_best[at] = key; s_second[at] = second; }
+          }
+        }
+        __syncthreads();
+        return s_count;
+      };
+      m = gather(t, 0ull);
+      if (m > kJoinThreads) {
+        // more than can be ranked: a threshold over all of them
+        t = max(t, from_float(block_threshold<kJoinThreads, unsigned int>(p.k, kJoinThreads, [&](unsigned int trial) {
+          int c = 0;
+          for (int i = threadIdx.x; i < n; i += kJoinThreads) c += as_float(s_key[i]) >= trial ? 1 : 0;
+          return c;
+        })));
+        m = gather(t, 0ull);
+      }
+      if (m > kJoinThreads) {
+        // Where more than can be ranked share the K-th key (beams that all are dead, rows of equal logits), the same search goes on
+        // over all bits of the keys, and then over what comes after the key.
+        auto at_least = [&](unsigned long long trial) {
+          int c = 0;
+          for (int i = threadIdx.x; i < n; i += kJoinThreads) c += s_key[i] >= trial ? 1 : 0;
+          return c;
+        };
+        t = max(1ull, block_threshold<kJoinThreads, unsigned long long>(p.k, kJoinThreads, at_least));
+        unsigned long long t2 = 0ull;
+        __shared__ int s_above;
+        if (threadIdx.x == 0) s_above = 0;
+        __syncthreads();
+        const int above_here = at_least(t + 1ull);
+        if (above_here > 0) atomicAdd(&s_above, above_here);
+        __syncthreads();
+        const int above = s_above;
+        if (above < p.k) {
+          t2 = block_threshold<kJoinThreads, unsigned long long>(p.k - above, kJoinThreads - above, [&](unsigned long long trial) {
+            int c = 0;
+            for (int i = threadIdx.x; i < n; i += kJoinThreads) c += (s_key[i] == t && second_of(i, s_key[i], __ldcg(elems + i)) >= trial) ? 1 : 0;
+            return c;
+          });
+        }
+        m = gather(t, t2);
+      }
+    }
+    if (one_each || (m > 64 && m > 2 * p.k)) {
+      // ranking compares each with each: a threshold over them first
+      const bool there = (int)threadIdx.x < m;
+      const unsigned long long key = one_each ? my_key : there ? s_best[threadIdx.x] : 0ull;
+      const unsigned long long second = one_each ? second_of(threadIdx.x, my_key, my_elem) : there ? s_second[threadIdx.x] : 0ull;
+      const bool any = key != 0ull;
+      const unsigned long long least = from_float(block_threshold_of<unsigned int>(p.k, p.k + p.k / 4, any, as_float(key)));
       __syncthreads();
       if (threadIdx.x == 0) s_count = 0;
       __syncthreads();
-      for (int i = threadIdx.x; i < n; i += kJoinThreads) {
-        const unsigned long long key = s_key[i];
-        if (key < t) continue;
-        const unsigned long long second = second_of(i, s_key[i], __ldcg(elems + i));
-        if (key > t || second >= t2) {
-          const int at = atomicAdd(&s_count, 1);
-          if (at < kJoinThreads) { s_best[at] = key; s_second[at] = second; }
+      if (any && key >= least) {
+        const int at = atomicAdd(&s_count, 1);
+        s_best[at] = key;
+        s_second[at] = second;
+      }
+      __syncthreads();
+      m = s_count;
+    }
+    rank_by_slices<kJoinThreads>(m, s_rank, [&](int i, int j) {
+      const unsigned long long a = s_best[i], b = s_best[j];
+      return a > b || (a == b && s_second[i] > s_second[j]);
+    });
+    if ((int)threadIdx.x < m && s_rank[threadIdx.x] < p.k) {
+      s_top[s_rank[threadIdx.x]] = s_best[threadIdx.x];
+      s_top_second[s_rank[threadIdx.x]] = s_second[threadIdx.x];
+    }
+    __syncthreads();
+    if (pass > 0 || p.beams == 1) break;
+
+    // ---- beams whose order the float exponentials may have wrong ----------------------------------------------------
+    const int last = min(m, p.k) - 1;
+    const double bound = order_bound(p.vocab);
+    auto top = [&](int i) { return from_ordered_f64(s_top[i]); };
+    auto beam_of = [&](unsigned long long second) { return kSelMaxBeams - 1 - (int)(second >> (32 + kSelTokenBits)); };
+    auto doubt = [&](int a, int b) { atomicOr(&s_doubt, 1ull << a | 1ull << b); };
+    for (int i = threadIdx.x; i < last; i += kJoinThreads) {         // of those that are wanted, two that are neighbours
+      const int a = beam_of(s_top_second[i]), b = beam_of(s_top_second[i + 1]);
+      if (a != b && top(i + 1) > -INFINITY && top(i) - top(i + 1) < bound) doubt(a, b);
+    }
+    if (top(last) > -INFINITY) {                                      // and those behind the last that is
+      const unsigned long long edge = ordered_f64(top(last) - bound);
+      auto look = [&](int i, unsigned long long key, unsigned long long elem) {
+        if (key < edge) return;
+        const unsigned long long second = second_of(i, key, elem);
+        if (key > s_top[last] || (key == s_top[last] && second >= s_top_second[last])) return;          // it is one of them
+        const int b = beam_of(second);
+        for (int j = last; j >= 0 && top(j) - from_ordered_f64(key) < bound; --j) {
+          if (beam_of(s_top_second[j]) != b) doubt(beam_of(s_top_second[j]), b);
+        }
+      };
+      if (one_each) {
+        look(threadIdx.x, my_key, my_elem);
+      } else {
+        for (int i = threadIdx.x; i < n; i += kJoinThreads) {
+          if (s_key[i / p.k * p.k] >= edge) look(i, s_key[i] != 0ull ? s_key[i] : any_key(i), __ldcg(elems + i));
         }
       }
-      __syncthreads();
-      return s_count;
-    };
-    m = gather(t, 0ull);
-    if (m > kJoinThreads) {
-      // more than can be ranked: a threshold over all of them
-      t = max(t, from_float(block_threshold<kJoinThreads, unsigned int>(p.k, kJoinThreads, [&](unsigned int trial) {
-        int c = 0;
-        for (int i = threadIdx.x; i < n; i += kJoinThreads) c += as_float(s_key[i]) >= trial ? 1 : 0;
-        return c;
-      })));
-      m = gather(t, 0ull);
     }
-    if (m > kJoinThreads) {
-      // Where more than can be ranked share the K-th key (beams that all are dead, rows of equal logits), the same search goes on
-      // over all bits of the keys, and then over what comes after the key.
-      auto at_least = [&](unsigned long long trial) {
-        int c = 0;
-        for (int i = threadIdx.x; i < n; i += kJoinThreads) c += s_key[i] >= trial ? 1 : 0;
-        return c;
-      };
-      t = max(1ull, block_threshold<kJoinThreads, unsigned long long>(p.k, kJoinThreads, at_least));
-      unsigned long long t2 = 0ull;
-      __shared__ int s_above;
-      if (threadIdx.x == 0) s_above = 0;
-      __syncthreads();
-      const int above_here = at_least(t + 1ull);
-      if (above_here > 0) atomicAdd(&s_above, above_here);
-      __syncthreads();
-      const int above = s_above;
-      if (above < p.k) {
-        t2 = block_threshold<kJoinThreads, unsigned long long>(p.k - above, kJoinThreads - above, [&](unsigned long long trial) {
-          int c = 0;
-          for (int i = threadIdx.x; i < n; i += kJoinThreads) c += (s_key[i] == t && second_of(i, s_key[i], __ldcg(elems + i)) >= trial) ? 1 : 0;
-          return c;
-        });
-      }
-      m = gather(t, t2);
+    __syncthreads();
+    const unsigned long long rows = s_doubt;
+    if (rows == 0ull) break;
+    for (int b = 0; b < p.beams; ++b) {
+      const double ref = s_ref[b];
+      if (!(rows >> b & 1ull) || ref == INFINITY) continue;           // (the sum of a row of +inf is exact)
+      const double sum = sum_again(p.logits + (long long)(row0 + b) * p.ld, p.vocab, ref, s_powers, s_part);
+      if (threadIdx.x == 0) s_log[b] = log(sum);
     }
   }
-  if (one_each || (m > 64 && m > 2 * p.k)) {
-    // ranking compares each with each: a threshold over them first
-    const bool there = (int)threadIdx.x < m;
-    const unsigned long long key = one_each ? my_key : there ? s_best[threadIdx.x] : 0ull;
-    const unsigned long long second = one_each ? second_of(threadIdx.x, my_key, my_elem) : there ? s_second[threadIdx.x] : 0ull;
-    const bool any = key != 0ull;
-    const unsigned long long least = from_float(block_threshold_of<unsigned int>(p.k, p.k + p.k / 4, any, as_float(key)));
-    __syncthreads();
-    if (threadIdx.x == 0) s_count = 0;
-    __syncthreads();
-    if (any && key >= least) {
-      const int at = atomicAdd(&s_count, 1);
-      s_best[at] = key;
-      s_second[at] = second;
-    }
-    __syncthreads();
-    m = s_count;
-  }
-  rank_by_slices<kJoinThreads>(m, s_rank, [&](int i, int j) {
-    const unsigned long long a = s_best[i], b = s_best[j];
-    return a > b || (a == b && s_second[i] > s_second[j]);
-  });
-  if ((int)threadIdx.x < m) {
-    const unsigned long long a = s_best[threadIdx.x], b = s_second[threadIdx.x];
-    const int rank = s_rank[threadIdx.x];
-    if (rank < p.k) {
-      const size_t at = (size_t)group * p.k + rank;
-      p.out_scores[at] = (float)from_ordered_f64(a);
-      p.out_parents[at] = kSelMaxBeams - 1 - (int)(b >> (32 + kSelTokenBits));
-      p.out_tokens[at] = (int)(kTokens - 1u - ((unsigned int)b & (kTokens - 1u)));
-    }
+  for (int i = threadIdx.x; i < p.k; i += kJoinThreads) {
+    const size_t at = (size_t)group * p.k + i;
+    const unsigned long long second = s_top_second[i];
+    p.out_scores[at] = (float)from_ordered_f64(s_top[i]);
+    p.out_parents[at] = kSelMaxBeams - 1 - (int)(second >> (32 + kSelTokenBits));
+    p.out_tokens[at] = (int)(kTokens - 1u - ((unsigned int)second & (kTokens - 1u)));
   }
 }
 

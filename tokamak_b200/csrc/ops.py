@@ -257,7 +257,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int, *, 
 
     ``logits`` are float32 ``[groups * beams, vocab]`` (rows may lie further apart), ``scores`` ``[groups, beams]`` the
     beams' sums of log probabilities.  A continuation's score is its beam's plus the log softmax of its logit; scores are
-    compared in 64 bits and rounded once.  Equal ones: the lower beam first, of one beam the larger logit, then the lower
+    compared in 64 bits (those of different beams to 4e-13) and returned as floats, off by their rounding and some 1e-7.  Equal ones: the lower beam first, of one beam the larger logit, then the lower
     token.  A beam with a score of -inf or NaN is not read; its continuations, with scores of -inf, come last, and so do
     logits of -inf or NaN.  ``out``: tensors to write to."""
     if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
