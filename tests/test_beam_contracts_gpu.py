@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_beam_kernels_gpu import BF16_HALF, DEV, F32_HALF, Shared, err_word, i32
+from test_beam_kernels_gpu import BF16_HALF, DEV, F32_HALF, Shared, err_word, i32, select_inputs, select_oracle
 from tokamak_b200.csrc import ops
 
 pytestmark = pytest.mark.gpu
@@ -141,3 +141,74 @@ def test_scores_that_nearly_are_equal_come_in_their_order(kind, beams, vocab, se
         got = ops.beam_select(torch.from_numpy(x).to(DEV), torch.from_numpy(s).to(DEV), k)
         np.testing.assert_array_equal(got[1].cpu().numpy(), parents[:, :k])
         np.testing.assert_array_equal(got[2].cpu().numpy(), tokens[:, :k])
+
+
+def test_sums_that_go_on_for_hundreds_of_steps():
+    """Selections and what follows from them, a step on the other, against the same in 64 bits on the host: which beams go on, with which
+    tokens, and their sums, as far as a row's logarithm is off (2e-13 a step) and a place of 64 bits near 4,000 (2^-41) a step."""
+    groups, beams, vocab, k, steps, stops = 3, 6, 2003, 18, 500, [5, 77]
+    rng = np.random.default_rng(8)
+    slots = i32(np.arange(groups * beams).reshape(groups, beams))
+    scores = torch.zeros(groups, beams, dtype=torch.float64, device=DEV)
+    scores[:, 1:] = -float("inf")
+    parents, tokens = torch.zeros_like(slots), torch.zeros_like(slots)
+    want = scores.cpu().numpy().copy()
+    stop_tokens, err = i32(stops), err_word()
+    for step in range(steps):
+        x = (rng.standard_normal((groups * beams, vocab)) * 2.0).astype(np.float32)
+        cand = ops.beam_select(torch.from_numpy(x).to(DEV), scores, k, score_dtype=torch.float64)
+        assert cand[0].dtype == torch.float64
+        ops.beam_advance(cand, stop_tokens, slots, scores, parents, tokens, err)
+        live = np.where(np.isfinite(want), want, -1e30)
+        keys, by, tok = ranked(x, live, k)
+        got = tuple(t.cpu().numpy() for t in cand)
+        np.testing.assert_array_equal(got[1], by)
+        np.testing.assert_array_equal(got[2], tok)
+        assert np.abs(got[0] - keys).max() <= (step + 1) * (2e-13 + 2.0 ** -41)
+        new = np.empty_like(want)
+        for g in range(groups):
+            seats, late = [None] * beams, []
+            for c in [c for c in range(k) if tok[g, c] not in stops][:beams]:
+                if seats[by[g, c]] is None:
+                    seats[by[g, c]] = c
+                else:
+                    late.append(c)
+            for c in late:
+                seats[seats.index(None)] = c
+            new[g] = keys[g][seats]
+            assert parents[g].tolist() == by[g][seats].tolist() and tokens[g].tolist() == tok[g][seats].tolist()
+        want = new
+        assert np.abs(scores.cpu().numpy() - want).max() <= (step + 1) * (2e-13 + 2.0 ** -41)
+    assert err.tolist()[0] == 0
+
+
+@pytest.mark.parametrize("kind", ["normal", "rising", "few_values", "masked", "nothing", "infinite", "dead", "far", "equal"])
+@pytest.mark.parametrize("groups,beams,vocab,k", [(2, 4, 30001, 8), (1, 1, 6, 6), (1, 64, 4099, 256), (145, 4, 9001, 8)])
+def test_selection_with_sums_in_64_bits(groups, beams, vocab, k, kind):
+    x, s = select_inputs(kind, groups, beams, vocab, seed=4)
+    s = s.astype(np.float64) + (0.0 if kind in ("equal", "few_values") else np.random.default_rng(1).random(s.shape) * 1e-9)
+    got = ops.beam_select(torch.from_numpy(x).to(DEV), torch.from_numpy(s).to(DEV), k, score_dtype=torch.float64)
+    for part in (slice(0, 2), slice(max(0, groups - 1), groups)):
+        rows = slice(part.start * beams, min(part.stop, groups) * beams)
+        keys, parents, tokens = select_oracle(x[rows], s[part], k)
+        scores = got[0][part].cpu().numpy()
+        finite = np.isfinite(keys)
+        assert np.array_equal(np.isneginf(scores), np.isneginf(keys))
+        # 1.5e-13 of a row's sum for the series, places of 64 bits (of keys up to some hundred) for the rest
+        assert np.abs(scores[finite] - keys[finite]).max(initial=0.0) <= 2e-13 + 2.0 ** -51 * np.abs(keys[finite]).max(initial=0.0)
+        np.testing.assert_array_equal(got[1][part].cpu().numpy(), parents)
+        np.testing.assert_array_equal(got[2][part].cpu().numpy(), tokens)
+
+
+def test_sums_of_another_type_are_refused():
+    x, s = torch.zeros(6, 50, device=DEV), torch.zeros(2, 3, device=DEV)
+    ints = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=DEV)
+    wide = (s.double()[:, :1].contiguous(), ints(2, 1), ints(2, 1))
+    for bad in (lambda: ops.beam_select(x, s, 4, score_dtype=torch.float64), lambda: ops.beam_select(x, s.double(), 4),
+                lambda: ops.beam_select(x, s.half(), 4, score_dtype=torch.float16),
+                lambda: ops.beam_select(x, s.double(), 4, score_dtype=torch.float64, out=(torch.zeros(2, 4, device=DEV), ints(2, 4), ints(2, 4))),
+                lambda: ops.beam_advance(wide, None, ints(2, 3), s, ints(2, 3), ints(2, 3), err_word()),
+                lambda: ops.beam_advance((wide[0].float(),) + wide[1:], None, ints(2, 3), s.double(), ints(2, 3), ints(2, 3), err_word()),
+                lambda: ops.beam_advance((wide[0].half(),) + wide[1:], None, ints(2, 3), s.half(), ints(2, 3), ints(2, 3), err_word())):
+        with pytest.raises(ops.KernelError):
+            bad()

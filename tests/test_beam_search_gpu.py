@@ -172,3 +172,30 @@ def test_searches_that_are_refused():
     small.cache_manager.kv_groups[0].allocator.num_pages = 20          # what the pool says it holds
     with pytest.raises(ValueError, match="kv_pool_tokens"):
         small.beam_search(prompt_token_ids=[[1] * 100], params=BeamSearchParams(beam_width=3, max_new_tokens=100))
+
+
+def test_sums_are_carried_in_64_bits(monkeypatch):
+    """What a step starts from is, to 2e-13, what the one before it returned plus a log probability in 64 bits, and so is what is reported."""
+    from tokamak_b200 import BeamSearchParams
+    from tokamak_b200.engine import beam
+    prompt, width, tokens = prompts_of("C", (40,))[0], 3, 60
+    llm = llm_for("C", "float32", width, 1)
+    llm.plain_steps = True
+    calls, select = [], beam.ops.beam_select
+
+    def recorded(logits, scores, candidates, **kw):
+        before = scores.clone()
+        out = select(logits, scores, candidates, **kw)
+        calls.append((logits.clone(), before, tuple(t.clone() for t in out)))
+        return out
+
+    monkeypatch.setattr(beam.ops, "beam_select", recorded)
+    found = llm.beam_search(prompt_token_ids=[prompt], params=BeamSearchParams(beam_width=width, max_new_tokens=tokens, ignore_eos=True))[0].hypotheses
+    assert len(calls) == tokens
+    for i, (logits, before, (scores, parents, chosen)) in enumerate(calls):
+        logp = torch.log_softmax(logits.double(), -1)
+        want = before.double()[0, parents[0].long()] + logp[parents[0].long(), chosen[0].long()]
+        assert float((scores[0].double() - want).abs().max()) <= 2e-13 + 2.0 ** -51 * float(want.abs().max())
+        if i > 0:
+            assert set(before[0].tolist()) <= set(calls[i - 1][2][0][0].tolist())
+    assert [h.cumulative_logprob for h in found] == calls[-1][2][0][0][:width].tolist()

@@ -47,10 +47,10 @@ constexpr float kSelRaise = 12.0f;                             // exponents abov
 
 struct SelectParams {
   const float* logits;          // [groups * beams, vocab], row stride ld
-  const float* scores;          // [groups, beams]
+  const void* scores;           // [groups, beams], of the type that the kernels are made for
   double* seg_sum;              // [rows, segments, 2]: reference, sum of exponentials
   unsigned long long* seg_key;  // [rows, segments, K]: ordered logit, then ~token; 0 behind the last
-  float* out_scores;            // [groups, K]
+  void* out_scores;             // [groups, K]
   int* out_parents;
   int* out_tokens;
   long long ld;
@@ -73,7 +73,7 @@ __device__ __forceinline__ double from_ordered_f64(unsigned long long o) {
   return __longlong_as_double((long long)((o >> 63) ? (o & 0x7fffffffffffffffull) : ~o));
 }
 
-__device__ __forceinline__ bool dead_score(float s) { return !(s > -INFINITY); }        // -inf or NaN
+__device__ __forceinline__ bool dead_score(double s) { return !(s > -INFINITY); }       // -inf or NaN
 
 // The largest threshold, bit by bit from the top, with at least k of the block's values at or above it; it stops early at one
 // with at most `most`.  count(t) gives this thread's values at or above t.
@@ -247,22 +247,24 @@ __device__ __forceinline__ void add_terms(double (&sum)[2], const float* x, floa
 // kPerSm: blocks on an SM at a time.  Four leave a thread 64 registers, and it keeps some of its values in memory; where there are
 // no more blocks than three an SM take (8 groups of 4 beams over 151,936 tokens: 416), they are faster by themselves: 15.3 us
 // against 17.0 for the selection.  512 rows of 100,003 logits, more than that: 68 us with three, 55 with four.
-template <int kPerSm>
+template <int kPerSm, typename Score>
 __global__ void __launch_bounds__(kSelThreads, kPerSm)
 beam_segments_kernel(SelectParams p) {
+  constexpr bool kWide = sizeof(Score) == 8;      // exponentials in 64 bits
   pdl_trigger();
   __shared__ unsigned long long s_buf[kSelBuffer];
   __shared__ int s_count, s_rank[kSelKept];
   __shared__ float s_max[kSelThreads / 32];
-  __shared__ double s_sum[kSelThreads / 32], s_late[kSelMaxK];
+  __shared__ double s_sum[kSelThreads / 32], s_late[kWide ? 1 : kSelMaxK], s_powers[16];
   const int seg = blockIdx.x;
   const long long row = blockIdx.y;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const size_t at_part = (size_t)row * p.segments + seg;
   unsigned long long* out = p.seg_key + at_part * p.k;
   const int begin = min(p.vocab, seg * p.seg_len), end = min(p.vocab, begin + p.seg_len);
+  if (kWide && threadIdx.x < 16) s_powers[threadIdx.x] = kPowers[threadIdx.x];
   pdl_wait();
-  if (dead_score(p.scores[row])) {
+  if (dead_score(((const Score*)p.scores)[row])) {
     // the first tokens stand for a beam that cannot go on
     for (int i = threadIdx.x; i < p.k; i += kSelThreads) {
       out[i] = (seg == 0 && i < p.vocab) ? ((unsigned long long)ordered_f32(-INFINITY) << 32) | (0xffffffffu - (unsigned)i) : 0ull;
@@ -358,15 +360,22 @@ beam_segments_kernel(SelectParams p) {
       sum = ref == -INFINITY ? 0.0 : sum * exp((double)ref - (double)m);
       ref = m;
     }
+    if constexpr (kWide) {
+      double two[2] = {sum, 0.0};
 #pragma unroll
-    for (int j = 0; j + 3 < kSelEach; j += 4) {
-      const float2 a = terms_f32(e[j], e[j + 1], ref), b = terms_f32(e[j + 2], e[j + 3], ref);
-      const float2 c = add2(a, b);
-      sum += (double)(c.x + c.y);
-    }
-    if (kSelEach % 4 == 2) {
-      const float2 a = terms_f32(e[kSelEach - 2], e[kSelEach - 1], ref);
-      sum += (double)(a.x + a.y);
+      for (int j = 0; j < kSelEach; j += 2) add_terms<2>(two, e + j, ref, (double)ref, s_powers);
+      sum = two[0] + two[1];
+    } else {
+#pragma unroll
+      for (int j = 0; j + 3 < kSelEach; j += 4) {
+        const float2 a = terms_f32(e[j], e[j + 1], ref), b = terms_f32(e[j + 2], e[j + 3], ref);
+        const float2 c = add2(a, b);
+        sum += (double)(c.x + c.y);
+      }
+      if (kSelEach % 4 == 2) {
+        const float2 a = terms_f32(e[kSelEach - 2], e[kSelEach - 1], ref);
+        sum += (double)(a.x + a.y);
+      }
     }
   };
   add_tile(cur, top);
@@ -425,8 +434,8 @@ beam_segments_kernel(SelectParams p) {
   if (!same) sum = (ref == -INFINITY || ref_all == INFINITY) ? 0.0 : sum * exp((double)ref - (double)ref_all);
   // Where no thread raised its reference, the K best, which the sum is mostly made of, are summed in 64 bits after all: what their
   // fast exponentials were off by is added.
-  const bool one_ref = __syncthreads_and(same) && ref_all > -INFINITY && ref_all < INFINITY;
-  if ((int)threadIdx.x < p.k) s_late[threadIdx.x] = 0.0;
+  const bool one_ref = !kWide && __syncthreads_and(same) && ref_all > -INFINITY && ref_all < INFINITY;
+  if (!kWide && (int)threadIdx.x < p.k) s_late[threadIdx.x] = 0.0;
   for (int i = threadIdx.x; i < kSelKept; i += kSelThreads) s_rank[i] = 0;
   __syncthreads();
   rank_by_slices<kSelThreads>(n, s_rank, [&](int i, int j) { return s_buf[i] > s_buf[j]; });
@@ -441,7 +450,7 @@ beam_segments_kernel(SelectParams p) {
   }
   for (int i = n + (int)threadIdx.x; i < p.k; i += kSelThreads) out[i] = 0ull;
   __syncthreads();
-  if ((int)threadIdx.x < p.k) sum += s_late[threadIdx.x];        // by rank: the order of the additions is always the same
+  if (!kWide && (int)threadIdx.x < p.k) sum += s_late[threadIdx.x];        // by rank: the order of the additions is always the same
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) s_sum[warp] = sum;
@@ -480,6 +489,7 @@ __device__ __noinline__ double sum_again(const float* x, int vocab, double ref, 
 
 // One block per group: the sums of its rows, the keys of the elements set aside, the K best of them in order.  A segment's elements
 // come best first, so where there are more segments than K only those whose first is among the K best firsts matter.
+template <typename Score>
 __global__ void __launch_bounds__(kJoinThreads, 2)
 beam_join_kernel(SelectParams p) {
   pdl_trigger();
@@ -521,7 +531,7 @@ beam_join_kernel(SelectParams p) {
   __syncthreads();
   auto key_of = [&](int b, unsigned long long elem) {
     const double x = (double)from_ordered_f32((unsigned int)(elem >> 32));
-    const double s = (double)p.scores[row0 + b];
+    const double s = (double)((const Score*)p.scores)[row0 + b];
     const double ref = s_ref[b];
     double key = s + ((ref == INFINITY ? (x == INFINITY ? 0.0 : -INFINITY) : x - ref) - s_log[b]);
     if (!(key > -INFINITY)) key = -INFINITY;                   // dead beams, -inf logits, rows of -inf alone
@@ -654,7 +664,7 @@ beam_join_kernel(SelectParams p) {
       s_top_second[s_rank[threadIdx.x]] = s_second[threadIdx.x];
     }
     __syncthreads();
-    if (pass > 0 || p.beams == 1) break;
+    if (pass > 0 || p.beams == 1 || sizeof(Score) == 8) break;
 
     // ---- beams whose order the float exponentials may have wrong ----------------------------------------------------
     const int last = min(m, p.k) - 1;
@@ -698,7 +708,7 @@ beam_join_kernel(SelectParams p) {
   for (int i = threadIdx.x; i < p.k; i += kJoinThreads) {
     const size_t at = (size_t)group * p.k + i;
     const unsigned long long second = s_top_second[i];
-    p.out_scores[at] = (float)from_ordered_f64(s_top[i]);
+    ((Score*)p.out_scores)[at] = (Score)from_ordered_f64(s_top[i]);
     p.out_parents[at] = kSelMaxBeams - 1 - (int)(second >> (32 + kSelTokenBits));
     p.out_tokens[at] = (int)(kTokens - 1u - ((unsigned int)second & (kTokens - 1u)));
   }
@@ -711,12 +721,12 @@ beam_join_kernel(SelectParams p) {
 // goes on is never written, and what has to move is one record for every beam that ends.  A seat that is left without a
 // candidate (a vocabulary of stop tokens) keeps its parent with a score of -inf.
 struct AdvanceParams {
-  const float* cand_scores;     // [groups, K], best first
+  const void* cand_scores;      // [groups, K], best first, of the type that the kernel is made for
   const int* cand_parents;
   const int* cand_tokens;
   const int* stop_tokens;       // [n_stop]
   const int* slots;             // [groups, beams]
-  float* scores;                // [groups, beams], rewritten
+  void* scores;                 // [groups, beams], rewritten
   int* parents;                 // [groups, beams]: the seat that each seat goes on from
   int* tokens;                  // [groups, beams]
   int* records;                 // [max_slots, words] or null: word `token_word` receives the token
@@ -727,8 +737,10 @@ struct AdvanceParams {
   int k, beams, n_stop, max_slots, words, token_word, history_ld, from_one;
 };
 
+template <typename Score>
 __global__ void __launch_bounds__(64) beam_advance_kernel(AdvanceParams p) {
   pdl_trigger();
+  const Score* cand_scores = (const Score*)p.cand_scores;
   __shared__ int s_cand[kSelMaxBeams];       // candidate of every seat, -1: none yet
   __shared__ int s_late[kSelMaxBeams];
   pdl_wait();
@@ -740,7 +752,7 @@ __global__ void __launch_bounds__(64) beam_advance_kernel(AdvanceParams p) {
   if (threadIdx.x == 0) {
     int taken = 0, late = 0;
     for (int i = 0; i < p.k && taken < p.beams; ++i) {
-      if (!(p.cand_scores[c0 + i] > -INFINITY)) break;          // what comes now cannot go on
+      if (!(cand_scores[c0 + i] > -INFINITY)) break;          // what comes now cannot go on
       const int tok = p.cand_tokens[c0 + i];
       bool stop = false;
       for (int j = 0; j < p.n_stop; ++j) stop = stop || p.stop_tokens[j] == tok;
@@ -764,7 +776,7 @@ __global__ void __launch_bounds__(64) beam_advance_kernel(AdvanceParams p) {
   const int token = c >= 0 ? p.cand_tokens[c0 + c] : 0;
   int parent = c >= 0 && !p.from_one ? p.cand_parents[c0 + c] : seat;
   if (parent < 0 || parent >= p.beams) { set_error(p.err, kErrRequest, g, parent, p.beams); parent = seat; }
-  p.scores[b0 + seat] = c >= 0 ? p.cand_scores[c0 + c] : -INFINITY;
+  ((Score*)p.scores)[b0 + seat] = c >= 0 ? cand_scores[c0 + c] : (Score)-INFINITY;
   p.parents[b0 + seat] = parent;
   p.tokens[b0 + seat] = token;
   const int slot = p.slots[b0 + seat];
@@ -909,8 +921,9 @@ __global__ void __launch_bounds__(kMoveThreads, kSeats <= 8 ? 6 : kSeats <= 32 ?
 }  // namespace tk
 
 // scratch: rows * segments * (16 + 8 k) bytes, on 8 bytes.
-TK_API int tk_beam_select(const float* logits, long long ld, const float* scores, void* scratch, float* out_scores,
-                          int* out_parents, int* out_tokens, int groups, int beams, int vocab, int k, int segments,
+// wide: scores and out_scores are doubles.
+TK_API int tk_beam_select(const float* logits, long long ld, const void* scores, void* scratch, void* out_scores,
+                          int* out_parents, int* out_tokens, int groups, int beams, int vocab, int k, int segments, int wide,
                           cudaStream_t stream) {
   if (groups <= 0) return 0;
   if (beams < 1 || beams > tk::kSelMaxBeams || k < 1 || k > tk::kSelMaxK || vocab < 1 || segments < 1 || ld < vocab ||
@@ -933,26 +946,31 @@ TK_API int tk_beam_select(const float* logits, long long ld, const float* scores
   if (e != cudaSuccess) return (int)e;
   if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidValue;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(tk::beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tk::kSelMaxEntries * 8);
+    e = cudaFuncSetAttribute(tk::beam_join_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, tk::kSelMaxEntries * 8);
+    if (e != cudaSuccess) return (int)e;
+    e = cudaFuncSetAttribute(tk::beam_join_kernel<double>, cudaFuncAttributeMaxDynamicSharedMemorySize, tk::kSelMaxEntries * 8);
     if (e != cudaSuccess) return (int)e;
     configured[dev] = true;
   }
   const bool few = (long long)segments * groups * beams <= 3LL * tk::device_sm_count();
-  e = tk::launch(few ? tk::beam_segments_kernel<3> : tk::beam_segments_kernel<4>, dim3(segments, groups * beams), dim3(tk::kSelThreads), 0,
-                 stream, p);
+  auto* first = wide ? (few ? tk::beam_segments_kernel<3, double> : tk::beam_segments_kernel<4, double>)
+                     : (few ? tk::beam_segments_kernel<3, float> : tk::beam_segments_kernel<4, float>);
+  e = tk::launch(first, dim3(segments, groups * beams), dim3(tk::kSelThreads), 0, stream, p);
   if (e != cudaSuccess) return (int)e;
-  return (int)tk::launch(tk::beam_join_kernel, dim3(groups), dim3(tk::kJoinThreads), join_smem, stream, p);
+  return (int)tk::launch(wide ? tk::beam_join_kernel<double> : tk::beam_join_kernel<float>, dim3(groups), dim3(tk::kJoinThreads), join_smem,
+                         stream, p);
 }
 
-TK_API int tk_beam_advance(const float* cand_scores, const int* cand_parents, const int* cand_tokens, const int* stop_tokens,
-                           const int* slots, float* scores, int* parents, int* tokens, int* records,
+// wide: the scores are doubles.
+TK_API int tk_beam_advance(const void* cand_scores, const int* cand_parents, const int* cand_tokens, const int* stop_tokens,
+                           const int* slots, void* scores, int* parents, int* tokens, int* records,
                            unsigned char* history, const int* positions, const int* prefix_len, int* err, int groups, int beams, int k, int n_stop,
-                           int max_slots, int words, int token_word, int history_ld, int from_one, cudaStream_t stream) {
+                           int max_slots, int words, int token_word, int history_ld, int from_one, int wide, cudaStream_t stream) {
   if (groups <= 0) return 0;
   if (beams < 1 || beams > tk::kSelMaxBeams || k < 1 || n_stop < 0) return (int)cudaErrorInvalidValue;
   tk::AdvanceParams p{cand_scores, cand_parents, cand_tokens, stop_tokens, slots, scores, parents, tokens, records, history,
                       positions, prefix_len, err, k, beams, n_stop, max_slots, words, token_word, history_ld, from_one};
-  return (int)tk::launch(tk::beam_advance_kernel, dim3(groups), dim3(64), 0, stream, p);
+  return (int)tk::launch(wide ? tk::beam_advance_kernel<double> : tk::beam_advance_kernel<float>, dim3(groups), dim3(64), 0, stream, p);
 }
 
 // tensors: address, bytes of a record and keys of each; a record's bytes and its tensor's address decide how wide its columns are.

@@ -139,8 +139,8 @@ _SIGNATURES: dict[str, list] = {
     "tk_gemm_f32_tile": [c_int, c_int, c_int, c_int],
     "tk_gemm_f32": [_P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong,
                     c_int, _P],
-    "tk_beam_select": [_P, c_longlong, _P, _P, _P, _P, _P] + 5 * [c_int] + [_P],
-    "tk_beam_advance": 13 * [_P] + 9 * [c_int] + [_P],
+    "tk_beam_select": [_P, c_longlong, _P, _P, _P, _P, _P] + 6 * [c_int] + [_P],
+    "tk_beam_advance": 13 * [_P] + 10 * [c_int] + [_P],
     "tk_reorder_slots": [_P, c_int, _P, _P, _P, c_int, c_int, c_int, _P],
     "tk_attention_shared_tc_takes": 5 * [c_int],
     "tk_attention_shared": 14 * [_P] + 15 * [c_int] + [c_float, c_float, c_int, _P],

@@ -250,14 +250,16 @@ def beam_segments(sms: int, rows: int, beams: int, vocab: int, candidates: int) 
     return min(range(1, most + 1), key=cost)
 
 
-def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int, *, out: tuple | None = None
-                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int, *, out: tuple | None = None,
+                score_dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The ``candidates`` best continuations of every group of beams, best first: ``(scores, parents, tokens)``, each
-    ``[groups, candidates]`` (float32, int32, int32).
+    ``[groups, candidates]`` (``score_dtype``, int32, int32).
 
     ``logits`` are float32 ``[groups * beams, vocab]`` (rows may lie further apart), ``scores`` ``[groups, beams]`` the
     beams' sums of log probabilities.  A continuation's score is its beam's plus the log softmax of its logit; scores are
-    compared in 64 bits (those of different beams to 4e-13) and returned as floats, off by their rounding and some 1e-7.  Equal ones: the lower beam first, of one beam the larger logit, then the lower
+    compared in 64 bits (those of different beams to 4e-13) and returned as floats, off by their rounding and some 1e-7.  A search
+    that goes on for many steps keeps its sums in 64 bits: with a ``score_dtype`` of float64 ``scores`` and what is returned are of
+    that type, every exponential is too, and a score is off by 2e-13.  Equal ones: the lower beam first, of one beam the larger logit, then the lower
     token.  A beam with a score of -inf or NaN is not read; its continuations, with scores of -inf, come last, and so do
     logits of -inf or NaN.  ``out``: tensors to write to."""
     if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
@@ -279,12 +281,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int, *, 
                           f"got {rows} x {vocab}")
     if rows > 1 and logits.stride(0) < vocab:
         raise KernelError("rows of logits overlap")
+    if score_dtype not in (torch.float32, torch.float64):
+        raise KernelError(f"scores are float32 or float64, not {score_dtype}")
     shape = (groups, candidates)
     if out is None:
-        out = (torch.empty(shape, dtype=torch.float32, device=logits.device),
+        out = (torch.empty(shape, dtype=score_dtype, device=logits.device),
                torch.empty(shape, dtype=torch.int32, device=logits.device),
                torch.empty(shape, dtype=torch.int32, device=logits.device))
-    _want_here((scores, torch.float32, "scores"), (out[0], torch.float32, "out scores"), (out[1], torch.int32, "out parents"),
+    _want_here((scores, score_dtype, "scores"), (out[0], score_dtype, "out scores"), (out[1], torch.int32, "out parents"),
                (out[2], torch.int32, "out tokens"))
     for t in out:
         if t.shape != shape:
@@ -295,7 +299,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, candidates: int, *, 
     scratch = torch.empty(rows * segments * (2 + candidates), dtype=torch.int64, device=logits.device)
     _check(_lib().tk_beam_select(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, scores.data_ptr(),
                                  scratch.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), groups, beams,
-                                 vocab, candidates, segments, _stream()), "beam_select")
+                                 vocab, candidates, segments, int(score_dtype == torch.float64), _stream()), "beam_select")
     return out
 
 
@@ -306,15 +310,16 @@ def beam_advance(candidates: tuple, stop_tokens: torch.Tensor | None, slots: tor
     """The beams that go on after :func:`beam_select`: of a group's candidates, in order, the first whose tokens are not in
     ``stop_tokens`` (int32), as many as it has beams.
 
-    Written for every seat (``[groups, beams]``): the beam's new score, the seat that it goes on from and its token.  A beam
+    Written for every seat (``[groups, beams]``): the beam's new score (of the candidates' type, float32 or float64), the seat that it goes on from and its token.  A beam
     stays in its parent's seat unless a better one took it; the rest fill the other seats in order, so a seat that goes
     on is never written by :func:`reorder_slots`.  A seat that is left over goes on from itself with a score of -inf and token 0.
     ``records`` (int32 ``[slots, words]``): word ``token_word`` of the record of each seat's slot (``slots`` ``[groups,
     beams]``) receives the token.  ``history`` (uint8 ``[slots, n]``): the place ``positions - prefix_len`` of each
     seat's row receives the seat (see :class:`SharedPrefix`); call :func:`reorder_slots` afterwards.  ``begin``: the candidates
     continue one row (a search that begins); every seat goes on from itself, and the history is left alone."""
-    _want_here((candidates[0], torch.float32, "candidate scores"), (candidates[1], torch.int32, "candidate parents"),
-               (candidates[2], torch.int32, "candidate tokens"), (slots, torch.int32, "slots"), (scores, torch.float32, "scores"),
+    kind = torch.float64 if candidates[0].dtype == torch.float64 else torch.float32
+    _want_here((candidates[0], kind, "candidate scores"), (candidates[1], torch.int32, "candidate parents"),
+               (candidates[2], torch.int32, "candidate tokens"), (slots, torch.int32, "slots"), (scores, kind, "scores"),
                (parents, torch.int32, "parents"), (tokens, torch.int32, "tokens"), (err, torch.int32, "err"))
     for t in candidates:
         if t.dim() != 2 or t.shape != candidates[0].shape:
@@ -352,7 +357,7 @@ def beam_advance(candidates: tuple, stop_tokens: torch.Tensor | None, slots: tor
     _check(_lib().tk_beam_advance(candidates[0].data_ptr(), candidates[1].data_ptr(), candidates[2].data_ptr(), _ptr(stop_tokens),
                                   slots.data_ptr(), scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _ptr(records),
                                   _ptr(history), _ptr(positions), _ptr(prefix_len), err.data_ptr(), groups, beams, k, n_stop,
-                                  max_slots, words, int(token_word), ld, int(begin), _stream()), "beam_advance")
+                                  max_slots, words, int(token_word), ld, int(begin), int(kind == torch.float64), _stream()), "beam_advance")
 
 
 _REORDER_TENSORS = 24             # tensors of one launch

@@ -113,22 +113,25 @@ class BeamBuffers:
         device = step.device
         i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=device)
         self.groups, self.width, self.candidates = groups, width, candidates
+        self.parts = (("cand_scores", candidates, torch.float64), ("scores", width, torch.float64), ("cand_parents", candidates, torch.int32),
+                      ("cand_tokens", candidates, torch.int32), ("parents", width, torch.int32), ("tokens", width, torch.int32))
         self.history = torch.zeros((step.manager.max_slots, -(-longest // 16) * 16), dtype=torch.uint8, device=device)
         self.group_start = torch.arange(groups + 1, dtype=torch.int32, device=device) * width
         self.prefix_slot, self.prefix_len = i32(groups), i32(groups)
-        # what the host reads of a step: for every search the ranked continuations, then the beams that go on (their scores are
-        # what the next step starts from)
-        self.words = i32(groups * (3 * candidates + 3 * width))
+        # what the host reads of a step: for every search the ranked continuations and the beams that go on, whose scores, in 64
+        # bits, are what the next step starts from
+        self.words = i32(groups * 4 * (candidates + width))
         self.hosts = [torch.zeros(4 + self.words.numel(), dtype=torch.int32).pin_memory() for _ in range(3)]
         self.turn = 0
 
-    def views(self, n: int) -> dict:
-        """The parts of ``words`` for ``n`` searches."""
-        k, w, at, out = self.candidates, self.width, 0, {}
-        for name, size, dtype in (("cand_scores", k, torch.float32), ("cand_parents", k, torch.int32), ("cand_tokens", k, torch.int32),
-                                  ("scores", w, torch.float32), ("parents", w, torch.int32), ("tokens", w, torch.int32)):
-            out[name] = self.words[at:at + n * size].view(dtype).view(n, size)
-            at += n * size
+    def views(self, n: int, words: torch.Tensor | None = None) -> dict:
+        """The parts of ``words`` (the device's, or a copy of them) for ``n`` searches."""
+        words = self.words if words is None else words
+        at, out = 0, {}
+        for name, size, dtype in self.parts:
+            taken = n * size * dtype.itemsize // 4
+            out[name] = words[at:at + taken].view(dtype).view(n, size)
+            at += taken
         out["used"] = at
         return out
 
@@ -192,8 +195,8 @@ class BeamRunner:
         device = self.step.device
         logits = self.prefill(searches)
         v = b.views(n)
-        ops.beam_select(logits, torch.zeros((n, 1), dtype=torch.float32, device=device), self.candidates,
-                        out=(v["cand_scores"], v["cand_parents"], v["cand_tokens"]))
+        ops.beam_select(logits, torch.zeros((n, 1), dtype=torch.float64, device=device), self.candidates,
+                        out=(v["cand_scores"], v["cand_parents"], v["cand_tokens"]), score_dtype=torch.float64)
         seats = []
         for s in searches:
             s.beams = [(s.index, i) for i in range(w)]
@@ -232,7 +235,8 @@ class BeamRunner:
         ops.decode_begin(st.buffers.updates, st.buffers.dec_slots, n * w, st.max_seq_len, st.buffers.dec_token_ids,
                          st.buffers.dec_positions, st.buffers.dec_kv_len, batch.err)
         logits = self.model.forward(batch)
-        cand = ops.beam_select(logits, v["scores"], self.candidates, out=(v["cand_scores"], v["cand_parents"], v["cand_tokens"]))
+        cand = ops.beam_select(logits, v["scores"], self.candidates, out=(v["cand_scores"], v["cand_parents"], v["cand_tokens"]),
+                               score_dtype=torch.float64)
         ops.beam_advance(cand, self.stop_tokens, slots, v["scores"], v["parents"], v["tokens"], batch.err,
                          records=self.cache.slot_records, history=b.history, positions=batch.positions, prefix_len=b.prefix_len)
         ops.reorder_slots(self.records, slots, v["parents"], batch.err)
@@ -291,16 +295,12 @@ class BeamRunner:
         """Read a step; whether a search ended with it."""
         pending.event.synchronize()
         self.step._raise_on_error(pending.host[:4].tolist())
-        n, k, w = len(pending.searches), self.candidates, self.width
-        words, at, cols = pending.host[4:], 0, []
-        for size, dtype in ((k, torch.float32), (k, None), (k, None), (w, torch.float32), (w, None), (w, None)):
-            part = words[at:at + n * size]
-            cols.append((part.view(dtype) if dtype else part).view(n, size).tolist())
-            at += n * size
+        cols = {name: part.tolist() for name, part in self.buffers.views(len(pending.searches), pending.host[4:]).items() if name != "used"}
         ended = False
         for i, s in enumerate(pending.searches):
             if not s.done:
-                s.take(self.params, self.stops, zip(cols[0][i], cols[1][i], cols[2][i]), list(zip(cols[3][i], cols[4][i], cols[5][i])))
+                s.take(self.params, self.stops, zip(*(cols[name][i] for name in ("cand_scores", "cand_parents", "cand_tokens"))),
+                       list(zip(*(cols[name][i] for name in ("scores", "parents", "tokens")))))
                 ended = ended or s.done
         return ended
 
