@@ -160,9 +160,10 @@ class BeamRunner:
         self.seen: dict = {}
         self.placed = 0                  # searches that the buffers hold
 
-    def start(self, params: BeamSearchParams, max_step_tokens: int) -> None:
-        """What one call asks for."""
-        self.params, self.max_step_tokens, self.steps = params, max_step_tokens, 0
+    def start(self, params: BeamSearchParams, max_step_tokens: int, plain: bool = False) -> None:
+        """What one call asks for.  ``plain``: no step is launched before the one before it has been read, and none is replayed; the
+        host writes every beam's position and token."""
+        self.params, self.max_step_tokens, self.plain, self.steps = params, max_step_tokens, plain, 0
 
     # ---- prompts ---------------------------------------------------------------------------------------------------
     def prefill(self, searches: list[Search]) -> torch.Tensor:
@@ -211,10 +212,14 @@ class BeamRunner:
         if self.cache._states:
             ops.reorder_slots(self.cache._states, slots, torch.zeros_like(slots), err)
         self.collect(self._read(searches, v["used"]))
+        self.write_records(searches)
+
+    def write_records(self, searches: list[Search]) -> None:
+        """Where every beam is and its last token, for the next step."""
         for s in searches:
             for beam, tokens in zip(s.beams, s.tokens):
                 self.cache.write_record(self.manager.slot(beam), temperature=0.0, top_k=0, top_p=1.0, seed=0,
-                                        computed=len(s.prompt), last_token=tokens[-1])
+                                        computed=self.manager.length(beam), last_token=tokens[-1])
 
     def place(self, searches: list[Search], order: list[int]) -> None:
         """Put what the device holds of the running searches in their order (``order``: where each was before)."""
@@ -246,6 +251,8 @@ class BeamRunner:
         """Start the step that brings every beam's token number ``done`` (one is there) to its next."""
         st, n, w, b = self.step, len(searches), self.width, self.buffers
         entries = [StepEntry(beam, None, [0]) for s in searches for beam in s.beams]
+        if self.plain:
+            self.write_records(searches)
         batch = st._build_from_state(entries)
         # the bounds are buckets, so that what the kernels plan from them changes rarely
         prefix = _bucket(max(len(s.prompt) for s in searches))
@@ -254,9 +261,9 @@ class BeamRunner:
                                         max_own=own, history=b.history)
         key = (n, batch.max_kv_len, prefix, own)
         graph = self.graphs.get(key)
-        if graph is None and st.use_graphs and st.graph_safe and self.seen.get(key, 0) >= 1:
+        if graph is None and st.use_graphs and st.graph_safe and not self.plain and self.seen.get(key, 0) >= 1:
             graph = self._capture(key, batch, n)
-        if graph is not None:
+        if graph is not None and not self.plain:
             graph["graph"].replay()
             st.graph_launches += graph["kernels"]
             st.graph_replays += 1
@@ -323,7 +330,7 @@ class BeamRunner:
                     pending = self.launch(running, done)
                     done += 1
                 ahead = None
-                if all(s.budget > done for s in running):
+                if not self.plain and all(s.budget > done for s in running):
                     # the next step needs nothing of this one that is not on the device
                     ahead = self.launch(running, done)
                     done += 1

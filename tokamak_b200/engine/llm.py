@@ -140,7 +140,8 @@ class LLM:
         self._beam_runner: tuple | None = None
         # A debugging aid: with plain_steps every step is laid out by the host (tokens included),
         # none is launched ahead of the one before it and none is replayed from a CUDA graph.  The
-        # tokens must not depend on it.
+        # tokens must not depend on it.  (A search over beams: sums, and where a beam's past lies, stay on the
+        # device all the same.)
         self.plain_steps = False
 
     # ---- tokenizer (text in and out only; the engine itself works on token ids) ---------
@@ -299,14 +300,10 @@ class LLM:
         if self._beam_runner is None or self._beam_runner[0] != shape:
             self._beam_runner = (shape, BeamRunner(self.core.step, *shape))      # kept with the graphs it has captured
         runner = self._beam_runner[1]
-        runner.start(params, min(self.max_num_batched_tokens, self.core.max_step_tokens))
-        graphs, self.core.step.use_graphs = self.core.step.use_graphs, self.core.step.use_graphs and not self.plain_steps
+        runner.start(params, min(self.max_num_batched_tokens, self.core.max_step_tokens), self.plain_steps)
         replays = self.core.step.graph_replays
-        try:
-            for wave in waves:
-                runner.run(wave)
-        finally:
-            self.core.step.use_graphs = graphs
+        for wave in waves:
+            runner.run(wave)
         self.last_stats = {"steps": runner.steps, "waves": len(waves), "graph_replays": self.core.step.graph_replays - replays,
                            "pages_free": [g.num_free for g in self.cache_manager.kv_groups]}
         decode = self.tokenizer.decode if self._has_tokenizer() else None
