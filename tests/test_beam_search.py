@@ -112,3 +112,16 @@ def test_models_whose_attention_cannot_read_shared_keys_are_refused():
     assert refuses_search(model(a=block(knows, KVPagesNeed(1, 8)), b=block(other, StateNeed((3,))))) is None
     assert "'b'" in refuses_search(model(a=block(knows, KVPagesNeed(1, 8)), b=block(other, KVPagesNeed(1, 8))))
     assert refuses_search(model(a=block(other, {"mixer": {"pages": KVPagesNeed(1, 8)}}))) is not None
+
+
+def test_segments_of_rows_of_logits():
+    """Within what the kernels hold, and on the kernel with registers for three blocks an SM wherever that costs least."""
+    from tokamak_b200.csrc import ops
+    sms = 148
+    for rows, beams, vocab, k in [(1, 1, 151936, 8), (1, 1, 1, 1), (32, 4, 151936, 8), (16, 4, 151936, 8), (24, 4, 151936, 8), (64, 64, 4096, 256),
+                                  (512, 16, 100003, 32), (65535, 1, 5, 5), (8, 8, 2 ** 21, 64)]:
+        n = ops.beam_segments(sms, rows, beams, vocab, k)
+        assert 1 <= n <= max(1, -(-vocab // 3584)) and beams * n * k <= max(16384, beams * k)
+    # 416 blocks of four tiles, three an SM, cost less than 480 of three, four an SM
+    assert ops.beam_segments(sms, 32, 4, 151936, 8) == 13
+    assert ops.beam_segments(sms, 512, 16, 100003, 32) == 1

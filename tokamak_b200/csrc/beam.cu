@@ -245,8 +245,9 @@ __device__ __forceinline__ void add_terms(double (&sum)[2], const float* x, floa
 }
 
 // kPerSm: blocks on an SM at a time.  Four leave a thread 64 registers, and it keeps some of its values in memory; where there are
-// no more blocks than three an SM take (8 groups of 4 beams over 151,936 tokens: 416), they are faster by themselves: 15.3 us
-// against 17.0 for the selection.  512 rows of 100,003 logits, more than that: 68 us with three, 55 with four.
+// no more blocks than three an SM take, they are faster by themselves: 8 groups of 4 beams over 151,936 tokens in 13 segments, 416 blocks,
+// 19.9 us against 21.8 (and 22.4 in 15 segments, 480 blocks, with four; inputs not in L2).  512 rows of 100,003 logits, more than that:
+// 68 us with three, 55 with four.  With 64-bit exponentials 20.0 against 24.0.
 template <int kPerSm, typename Score>
 __global__ void __launch_bounds__(kSelThreads, kPerSm)
 beam_segments_kernel(SelectParams p) {

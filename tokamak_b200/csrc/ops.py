@@ -242,11 +242,16 @@ BEAM_SEAT_LIMIT = 64              # seats of a group that reorder_slots moves be
 
 @lru_cache(maxsize=None)
 def beam_segments(sms: int, rows: int, beams: int, vocab: int, candidates: int) -> int:
-    """Segments that a row of logits is cut into.  Four blocks run on an SM at a time; a block costs its tiles and, for the first
-    threshold and the ranks, about as much as 6,000 logits more.  Taken is the number for which the rounds of blocks cost least, none
-    shorter than a block's tile, and no more than the joining kernel holds the candidates of."""
+    """Segments that a row of logits is cut into.  Up to three blocks an SM run on a kernel that has registers for all they hold, more
+    on one with room for four, where each takes about a third longer; a block costs its tiles and, for the first threshold and the
+    ranks, about as much as 6,000 logits more.  Taken is the number for which the rounds of blocks cost least (of equal ones the
+    largest), none shorter than a block's tile, and no more than the joining kernel holds the candidates of."""
     most = max(1, min(-(-vocab // _BEAM_TILE), _BEAM_MAX_ENTRIES // (beams * candidates)))
-    cost = lambda s: -(-rows * s // (4 * sms)) * (-(-vocab // s // _BEAM_TILE) * _BEAM_TILE + 6000)
+
+    def cost(s: int) -> tuple[int, int]:
+        block = -(-vocab // s // _BEAM_TILE) * _BEAM_TILE + 6000
+        return (3 * block if rows * s <= 3 * sms else 4 * block * -(-rows * s // (4 * sms))), -s
+
     return min(range(1, most + 1), key=cost)
 
 
