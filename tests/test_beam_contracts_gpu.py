@@ -212,3 +212,17 @@ def test_sums_of_another_type_are_refused():
                 lambda: ops.beam_advance((wide[0].half(),) + wide[1:], None, ints(2, 3), s.half(), ints(2, 3), ints(2, 3), err_word())):
         with pytest.raises(ops.KernelError):
             bad()
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 32)])
+def test_scales_and_caps_that_are_none_are_refused(dtype, d):
+    """The maximum of the scores is taken before they are scaled."""
+    c = Shared([3], [90], 20, d=d, dtype=dtype, seed=3).device()
+    for bad in (dict(scale=0.0), dict(scale=-0.125), dict(scale=float("nan")), dict(scale=float("inf")), dict(softcap=-5.0),
+                dict(softcap=float("nan")), dict(softcap=float("inf"))):
+        with pytest.raises(ops.KernelError):
+            ops.attention_shared(c.dq, c.out, c.dk, c.dv_, c.shared(), *c.args, **{**c.kw, **bad})
+    assert bool(torch.isnan(c.out).all())
+    c.kw["softcap"] = 0.0                      # no cap
+    c.call()
+    c.check()

@@ -2064,7 +2064,7 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
     Row ``r`` of ``q`` ``[rows, Hq, d]`` is the token at ``positions[r]`` of the request in slot ``req_slot[r]``; it sees the
     positions up to its own (the last ``window`` of them), the shared ones read once for all members of its group.  Caches
     ``[pages, Hkv, page, d]`` (values ``dv``) and ``block_table`` ``[slots, pages]`` as in the other attention kernels, float32
-    or bfloat16; ``softcap`` and ``sinks`` as in :func:`attention_plain`.  Cached keys and values must be finite wherever
+    or bfloat16; ``softcap`` and ``sinks`` as in :func:`attention_plain`, ``scale`` is positive.  Cached keys and values must be finite wherever
     a member of the group sees them."""
     kind, i32 = q.dtype, torch.int32
     dtype = dtype_code(kind)
@@ -2093,6 +2093,8 @@ def attention_shared(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, 
         raise KernelError("a step needs a group, a member, and an own position at least")
     if window is not None and window < 1:
         raise KernelError(f"a window of {window} positions is none")
+    if not 0.0 < scale < math.inf or (softcap is not None and not 0.0 <= softcap < math.inf):
+        raise KernelError(f"scores are scaled by a positive number and capped at one, got {scale} and {softcap}")
     history, ld = shared.history, 0
     if history is not None:
         _want_here((history, torch.uint8, "history"))
