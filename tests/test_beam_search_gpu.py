@@ -289,3 +289,16 @@ def test_every_beams_logits_in_bfloat16(tag, monkeypatch):
         for i, t in enumerate(tokens):
             assert_logits_close(rows[i:i + 1], _last_logits(folder, tag, tuple(prompts[i // width] + t))[None], "bfloat16", f"step {step}, beam {i}")
     assert moved > 0                            # beams did change seats
+
+
+def test_as_many_eos_tokens_as_there_are_candidates_for():
+    from tokamak_b200 import BeamSearchParams
+    eos = tuple(range(3, 43))                   # forty: 3 * 41 candidates, but not 32 * 41
+    prompt = prompts_of("C", (20,))[0]
+    llm = llm_for("C", "float32", 32, 1, eos)
+    out = llm.beam_search(prompt_token_ids=[prompt], params=BeamSearchParams(beam_width=3, max_new_tokens=6))[0]
+    want, _ = plain_search("C", "float32", prompt, width=3, max_new=6, stops=eos)
+    assert [h.output_token_ids for h in out.hypotheses] == [t for t, _, _ in want]
+    with pytest.raises(ValueError, match="EOS tokens"):
+        llm.beam_search(prompt_token_ids=[prompt], params=BeamSearchParams(beam_width=32, max_new_tokens=6))
+    assert llm.beam_search(prompt_token_ids=[prompt], params=BeamSearchParams(beam_width=32, max_new_tokens=6, ignore_eos=True))

@@ -31,7 +31,10 @@ from ..models.decoder import flat_needs
 from ..sampling.beam import BeamSearchParams
 from .step import StepBatch, StepEntry, StepFunction, _bucket
 
-STOPS_MAX = ops.BEAM_MAX_CANDIDATES // 32 - 1     # EOS tokens for which there are candidates enough at any width
+
+def stops_max(width: int) -> int:
+    """EOS tokens for which there are candidates enough: were all of them ranked first in every beam, ``width`` others must be left."""
+    return ops.BEAM_MAX_CANDIDATES // width - 1
 
 
 def refuses_search(model) -> str | None:

@@ -260,7 +260,7 @@ class LLM:
         ``max_batch_size`` slots and the pages of its prompt and of every beam's continuation at its longest; searches that do
         not fit side by side run one after the other.  Refused for models with attention that cannot read shared keys
         and for more EOS tokens than there are candidates for."""
-        from .beam import STOPS_MAX, BeamRunner, Search, refuses_search
+        from .beam import BeamRunner, Search, refuses_search, stops_max
         params = params or BeamSearchParams()
         texts, token_lists = self._token_lists(prompts, prompt_token_ids)
         why = refuses_search(self.model)
@@ -270,8 +270,8 @@ class LLM:
         if width + 1 > slots:
             raise ValueError(f"a search of {width} beams takes {width + 1} slots, the engine has {slots}: raise max_batch_size")
         stops = () if params.ignore_eos else tuple(self.model_config.eos_token_ids)
-        if len(stops) > STOPS_MAX:
-            raise ValueError(f"beam_search takes up to {STOPS_MAX} EOS tokens, the model has {len(stops)}")
+        if len(stops) > stops_max(width):
+            raise ValueError(f"a search of {width} beams takes up to {stops_max(width)} EOS tokens, the model has {len(stops)}: lower beam_width")
         searches, pages = [], []
         for i, ids in enumerate(token_lists):
             if not ids:
