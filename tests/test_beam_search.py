@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import math
+import random
 import types
 
 import pytest
@@ -125,3 +126,21 @@ def test_segments_of_rows_of_logits():
     # 416 blocks of four tiles, three an SM, cost less than 480 of three, four an SM
     assert ops.beam_segments(sms, 32, 4, 151936, 8) == 13
     assert ops.beam_segments(sms, 512, 16, 100003, 32) == 1
+
+
+def test_the_host_keeps_a_tree_of_tokens():
+    """A step adds a node for every beam and copies none of what the beams have behind them."""
+    from tokamak_b200.engine.beam import Search
+    params, width, steps = BeamSearchParams(beam_width=4, max_new_tokens=4000), 4, 3000
+    s, want = Search(0, [1], 4000), [[] for _ in range(width)]
+    rng = random.Random(3)
+    for n in range(steps):
+        parents = [rng.randrange(width) if n else 0 for _ in range(width)]
+        seats = [(-0.1 * n - 0.01 * i, p, 10 * n + i) for i, p in enumerate(parents)]
+        before = s.heads
+        s.take(params, frozenset(), seats, seats)
+        if n:
+            assert all(head[0] is before[p] for head, p in zip(s.heads, parents))
+        want = [want[p] + [10 * n + i] for i, p in enumerate(parents)]
+    assert s.tokens == want and s.length == steps
+    assert [h.tokens for h in s.hypotheses(params)] == want

@@ -59,6 +59,15 @@ class Hypothesis:
         return self.sum_logprobs / len(self.tokens) ** length_penalty
 
 
+def path(node) -> list[int]:
+    """Tokens from the root of a tree to ``node``, which is ``(parent, token)``, or ``None`` for the root."""
+    out = []
+    while node is not None:
+        node, token = node
+        out.append(token)
+    return out[::-1]
+
+
 @dataclass
 class Search:
     """One prompt's search as the host keeps it."""
@@ -67,7 +76,8 @@ class Search:
     prompt: list[int]
     budget: int                         # most tokens that may be generated
     beams: list = field(default_factory=list)        # request ids of the beams, seat by seat
-    tokens: list[list[int]] = field(default_factory=list)     # tokens of every running beam, seat by seat
+    heads: list = field(default_factory=list)        # last node of every running beam in the tree of tokens, seat by seat
+    length: int = 0                     # tokens of a running beam
     scores: list[float] = field(default_factory=list)
     ended: list[Hypothesis] = field(default_factory=list)
     done: bool = False
@@ -75,6 +85,11 @@ class Search:
     @property
     def prompt_id(self):
         return ("prompt", self.index)
+
+    @property
+    def tokens(self) -> list[list[int]]:
+        """Tokens of every running beam, seat by seat."""
+        return [path(head) for head in self.heads]
 
     def take(self, params: BeamSearchParams, stops: frozenset, candidates, seats) -> None:
         """One step's ranked continuations and the beams that go on: ended ones become hypotheses."""
@@ -84,14 +99,13 @@ class Search:
             if running == width or score == -math.inf:
                 break                    # what ranks behind the last beam that goes on does not end a hypothesis either
             if token in stops:
-                past = self.tokens[parent] if self.tokens else []
-                self.ended.append(Hypothesis(past + [token], score, True))
+                self.ended.append(Hypothesis(path((self.heads[parent] if self.heads else None, token)), score, True))
             else:
                 running += 1
-        past = self.tokens or [[] for _ in range(width)]
-        self.tokens = [past[parent] + [token] for _, parent, token in seats]
+        past = self.heads or [None] * width
+        self.heads = [(past[parent], token) for _, parent, token in seats]
         self.scores = [score for score, _, _ in seats]
-        length = len(self.tokens[0])
+        self.length = length = self.length + 1
         rank = lambda h: -h.score(params.length_penalty)
         self.ended = sorted(self.ended, key=rank)[:width]
         best = max(self.scores)
@@ -104,7 +118,7 @@ class Search:
     def hypotheses(self, params: BeamSearchParams) -> list[Hypothesis]:
         """The best hypotheses, ended or cut off at the cap on tokens, best first."""
         out = list(self.ended)
-        if len(out) < params.beam_width or len(self.tokens[0]) >= self.budget:
+        if len(out) < params.beam_width or self.length >= self.budget:
             out += [Hypothesis(t, s, False) for t, s in zip(self.tokens, self.scores) if s > -math.inf]
         return sorted(out, key=lambda h: -h.score(params.length_penalty))[:params.beam_width]
 
@@ -220,9 +234,9 @@ class BeamRunner:
     def write_records(self, searches: list[Search]) -> None:
         """Where every beam is and its last token, for the next step."""
         for s in searches:
-            for beam, tokens in zip(s.beams, s.tokens):
+            for beam, (_, token) in zip(s.beams, s.heads):
                 self.cache.write_record(self.manager.slot(beam), temperature=0.0, top_k=0, top_p=1.0, seed=0,
-                                        computed=self.manager.length(beam), last_token=tokens[-1])
+                                        computed=self.manager.length(beam), last_token=token)
 
     def place(self, searches: list[Search], order: list[int]) -> None:
         """Put what the device holds of the running searches in their order (``order``: where each was before)."""
