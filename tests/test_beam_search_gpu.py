@@ -253,7 +253,7 @@ def test_searches_that_grow_into_the_next_bucket(tag):
     for dtype in ("float32", "bfloat16"):
         llm = llm_for(tag, dtype, 3, 2)
         first = llm.beam_search(prompt_token_ids=prompts, params=params)
-        graphs = llm._beam_runner[1].graphs
+        graphs = llm._beam_runner.graphs
         assert len({key[1] for key in graphs}) == 2 and llm.last_stats["graph_replays"] >= 30
         again = llm.beam_search(prompt_token_ids=prompts, params=params)
         llm.plain_steps = True
@@ -302,3 +302,23 @@ def test_as_many_eos_tokens_as_there_are_candidates_for():
     with pytest.raises(ValueError, match="EOS tokens"):
         llm.beam_search(prompt_token_ids=[prompt], params=BeamSearchParams(beam_width=32, max_new_tokens=6))
     assert llm.beam_search(prompt_token_ids=[prompt], params=BeamSearchParams(beam_width=32, max_new_tokens=6, ignore_eos=True))
+
+
+def test_graphs_outlive_another_number_of_prompts():
+    """Fewer prompts or tokens run on what is there; more make room for both."""
+    from tokamak_b200 import BeamSearchParams
+    prompts, found = prompts_of("C", (16, 40, 9, 33)), lambda outs: [[h.output_token_ids for h in o.hypotheses] for o in outs]
+    params = lambda n: BeamSearchParams(beam_width=3, max_new_tokens=n, ignore_eos=True)
+    llm = llm_for("C", "float32", 3, 4)
+    runners, graphs = [], []
+    for some, tokens in ((slice(0, 2), 12), (slice(0, 1), 12), (slice(1, 3), 7), (slice(0, 2), 12), (slice(0, 4), 5), (slice(2, 4), 12), (slice(0, 1), 20)):
+        got = llm.beam_search(prompt_token_ids=prompts[some], params=params(tokens))
+        fresh = llm_for("C", "float32", 3, 4)
+        assert found(got) == found(fresh.beam_search(prompt_token_ids=prompts[some], params=params(tokens)))
+        runners.append(llm._beam_runner)
+        graphs.append(len(llm._beam_runner.graphs))
+    first, wider, longer = runners[0], runners[4], runners[6]
+    assert runners == [first] * 4 + [wider] * 2 + [longer] and len({id(r) for r in runners}) == 3
+    assert (wider.buffers.groups, wider.longest, longer.buffers.groups, longer.longest) == (4, 12, 4, 20)
+    assert graphs[1] >= graphs[0] and graphs[3] == graphs[2]             # the fourth call replays what the first has captured
+    assert llm.beam_search(prompt_token_ids=prompts[:1], params=BeamSearchParams(beam_width=2, max_new_tokens=5)) and llm._beam_runner.width == 2

@@ -177,6 +177,10 @@ class BeamRunner:
         self.seen: dict = {}
         self.placed = 0                  # searches that the buffers hold
 
+    def takes(self, width: int, stops, groups: int, longest: int) -> bool:
+        """Whether its buffers, and the graphs that hold their addresses, do for searches of this kind."""
+        return (width == self.width and frozenset(stops) == self.stops and groups <= self.buffers.groups and longest <= self.longest)
+
     def start(self, params: BeamSearchParams, max_step_tokens: int, plain: bool = False) -> None:
         """What one call asks for.  ``plain``: no step is launched before the one before it has been read, and none is replayed; the
         host writes every beam's position and token."""

@@ -137,7 +137,7 @@ class LLM:
         self.model = self.core.model
         self._tokenizer = None
         self.last_stats: dict = {}
-        self._beam_runner: tuple | None = None
+        self._beam_runner = None                 # engine/beam.py's BeamRunner
         # A debugging aid: with plain_steps every step is laid out by the host (tokens included),
         # none is launched ahead of the one before it and none is replayed from a CUDA graph.  The
         # tokens must not depend on it.  (A search over beams: sums, and where a beam's past lies, stay on the
@@ -296,10 +296,12 @@ class LLM:
                 left = [g.num_pages for g in self.cache_manager.kv_groups]
             waves[-1].append(s)
             left = [a - b for a, b in zip(left, need)]
-        shape = (params.beam_width, stops, max(len(wave) for wave in waves), max(s.budget for s in searches))
-        if self._beam_runner is None or self._beam_runner[0] != shape:
-            self._beam_runner = (shape, BeamRunner(self.core.step, *shape))      # kept with the graphs it has captured
-        runner = self._beam_runner[1]
+        runner = self._beam_runner
+        groups, longest = max(len(wave) for wave in waves), max(s.budget for s in searches)
+        if runner is None or not runner.takes(width, stops, groups, longest):
+            if runner is not None and runner.width == width:                 # room for what it had room for
+                groups, longest = max(groups, runner.buffers.groups), max(longest, runner.longest)
+            runner = self._beam_runner = BeamRunner(self.core.step, width, stops, groups, longest)      # kept with the graphs it captures
         runner.start(params, min(self.max_num_batched_tokens, self.core.max_step_tokens), self.plain_steps)
         replays = self.core.step.graph_replays
         for wave in waves:
