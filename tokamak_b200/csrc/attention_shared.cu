@@ -53,6 +53,14 @@ __device__ __forceinline__ void load_rows(int longest, bool wide, int lane, Len 
   }
 }
 
+// A score in units of log2(e), capped by cap tanh(x / cap).  In float32 with tanhf: what capped_score_log2's fast exponential and division
+// leave, a few 1e-7 of the cap, is 1e-6 of a result, where float32 products and sums alone leave 3e-7.
+template <typename T>
+__device__ __forceinline__ float shared_score_log2(const SharedParams& p, float dot) {
+  if (sizeof(T) == 4 && p.cap_log2 != 0.0f) return p.cap_log2 * tanhf(dot * p.inv_cap);
+  return capped_score_log2(dot, p.scale_log2, p.cap_log2, p.inv_cap);
+}
+
 template <typename T, int kChunks>       // kChunks: 128-column chunks of a value row
 __global__ void __launch_bounds__(kShThreads) shared_parts_kernel(SharedParams p, int shared_tiles, int own_tiles, int n_shared_blocks) {
   pdl_trigger();
@@ -178,7 +186,7 @@ __global__ void __launch_bounds__(kShThreads) shared_parts_kernel(SharedParams p
       for (int r = 0; r < 4; ++r) {
         const int i = 4 * warp + r;
         const bool seen = i < n_pairs && s_row[lane] >= 0 && key <= s_pos[i] && key >= s_lo[i];
-        const float x = seen ? capped_score_log2(s[r], p.scale_log2, p.cap_log2, p.inv_cap) : -INFINITY;
+        const float x = seen ? shared_score_log2<T>(p, s[r]) : -INFINITY;
         const float m_new = fmaxf(m[r], warp_max(x));
         const float m_use = m_new == -INFINITY ? 0.0f : m_new;
         const float corr = exp2f(m[r] - m_use);
