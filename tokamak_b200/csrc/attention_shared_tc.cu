@@ -864,7 +864,8 @@ constexpr int own_smem(int per) {
 
 // STAGES: tiles of a warp on their way or in use.  With a history most positions behind the prefix are common to a group, few are
 // left to a row, and what counts is how many rows are under way: one stage, four blocks on an SM (62 us against 67 for 16 groups of 4,
-// 113 against 119 for 4 of 16).  Without one all of them are the rows' own: two stages, three blocks (58 us against 73 for 48 rows
+// 113 against 119 for 4 of 16, measured, as all in these comments but the times of whole calls, before probabilities were two bfloat16).
+// Without one all of them are the rows' own: two stages, three blocks (58 us against 73 for 48 rows
 // with up to 700).
 template <int D, int STAGES>
 __global__ void __launch_bounds__(kSoWarps * 32, STAGES == 1 ? 4 : 3)
