@@ -256,3 +256,29 @@ def test_float32_shared_attention_is_as_good_as_float32(softcap, history):
     want = c.oracle()[0]
     rms = lambda x: float((x - want).pow(2).mean().sqrt())
     assert rms(c.out.cpu().double()) <= 1.5 * rms(in_float32(c))
+
+
+def test_nearly_equal_scores_in_one_group_of_several_and_in_a_graph():
+    """Rows that lie apart at any address; what one replay found in doubt is nothing to the next."""
+    groups, beams, vocab, k = 3, 8, 20011, 12
+    cases = []
+    for seed in (11, 12):
+        x, s = select_inputs("normal", groups, beams, vocab, seed=seed)
+        x[beams:2 * beams], s[1:2] = nearly_equal("normal", beams, vocab, seed)
+        cases.append((x, s) + ranked(x, s, k))
+        gaps = np.abs(np.diff(cases[-1][2], axis=1))
+        assert gaps.min() > 4e-13 and gaps[1].min() < 1e-8 < 1e-5 < gaps[[0, 2]].min()
+    memory = torch.full((3 + groups * beams * (vocab + 5),), float("nan"), device=DEV)
+    logits = memory[3:].view(groups * beams, vocab + 5)[:, :vocab]
+    scores = torch.zeros(groups, beams, device=DEV)
+    graph, out = torch.cuda.CUDAGraph(), None
+    ops.beam_select(logits, scores, k)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = ops.beam_select(logits, scores, k)
+    for x, s, _, parents, tokens in cases + cases[:1]:
+        logits.copy_(torch.from_numpy(x))
+        scores.copy_(torch.from_numpy(s))
+        graph.replay()
+        np.testing.assert_array_equal(out[1].cpu().numpy(), parents)
+        np.testing.assert_array_equal(out[2].cpu().numpy(), tokens)

@@ -554,12 +554,13 @@ beam_join_kernel(SelectParams p) {
     return ((unsigned long long)(kSelMaxBeams - 1 - i / per_row) << (32 + kSelTokenBits)) |
            ((unsigned long long)logit << kSelTokenBits) | (kTokens - 1u - token);
   };
-  // twice where the first time leaves it in doubt which of two beams' continuations is ranked higher
-  for (int pass = 0;; ++pass) {
+  // The K best in order, by the sums as they are.  Returns how many there are.
+  unsigned long long my_key = 0ull;
+  auto rank_all = [&]() -> int {
     s_rank[threadIdx.x] = 0;
     if (threadIdx.x == 0) s_count = 0;
     __syncthreads();
-    const unsigned long long my_key = my_elem == 0ull ? 0ull : key_of((int)threadIdx.x / per_row, my_elem);
+    my_key = my_elem == 0ull ? 0ull : key_of((int)threadIdx.x / per_row, my_elem);
     int m = 0;
     if (!one_each) {
       unsigned long long t = 1ull;                                   // everything there is
@@ -665,39 +666,64 @@ beam_join_kernel(SelectParams p) {
       s_top_second[s_rank[threadIdx.x]] = s_second[threadIdx.x];
     }
     __syncthreads();
-    if (pass > 0 || p.beams == 1 || sizeof(Score) == 8) break;
+    return min(m, p.k);
+  };
 
-    // ---- beams whose order the float exponentials may have wrong ----------------------------------------------------
-    const int last = min(m, p.k) - 1;
+  // ---- beams whose order the float exponentials may have wrong: a bit each -------------------------------------------
+  auto in_doubt = [&](int last) -> unsigned long long {
     const double bound = order_bound(p.vocab);
     auto top = [&](int i) { return from_ordered_f64(s_top[i]); };
+    const unsigned long long all = ~0ull >> (kSelMaxBeams - p.beams);
     auto beam_of = [&](unsigned long long second) { return kSelMaxBeams - 1 - (int)(second >> (32 + kSelTokenBits)); };
-    auto doubt = [&](int a, int b) { atomicOr(&s_doubt, 1ull << a | 1ull << b); };
+    unsigned long long rows = 0ull;                                   // a bit a beam
     for (int i = threadIdx.x; i < last; i += kJoinThreads) {         // of those that are wanted, two that are neighbours
       const int a = beam_of(s_top_second[i]), b = beam_of(s_top_second[i + 1]);
-      if (a != b && top(i + 1) > -INFINITY && top(i) - top(i + 1) < bound) doubt(a, b);
+      if (a != b && top(i + 1) > -INFINITY && top(i) - top(i + 1) < bound) rows |= 1ull << a | 1ull << b;
     }
     if (top(last) > -INFINITY) {                                      // and those behind the last that is
       const unsigned long long edge = ordered_f64(top(last) - bound);
+      // returns whether the element is one of them
       auto look = [&](int i, unsigned long long key, unsigned long long elem) {
-        if (key < edge) return;
+        if (key < edge) return false;
         const unsigned long long second = second_of(i, key, elem);
-        if (key > s_top[last] || (key == s_top[last] && second >= s_top_second[last])) return;          // it is one of them
+        if (key > s_top[last] || (key == s_top[last] && second >= s_top_second[last])) return true;
         const int b = beam_of(second);
-        for (int j = last; j >= 0 && top(j) - from_ordered_f64(key) < bound; --j) {
-          if (beam_of(s_top_second[j]) != b) doubt(beam_of(s_top_second[j]), b);
+        for (int j = last; j >= 0 && rows != all && top(j) - from_ordered_f64(key) < bound; --j) {
+          const int a = beam_of(s_top_second[j]);
+          if (a != b) rows |= 1ull << a | 1ull << b;
         }
+        return false;
       };
       if (one_each) {
         look(threadIdx.x, my_key, my_elem);
       } else {
-        for (int i = threadIdx.x; i < n; i += kJoinThreads) {
-          if (s_key[i / p.k * p.k] >= edge) look(i, s_key[i] != 0ull ? s_key[i] : any_key(i), __ldcg(elems + i));
+        // of every list, best first, the first that is none of them: whoever is close to a later one is close to it
+        for (int l = threadIdx.x; l < lists; l += kJoinThreads) {
+          const unsigned long long* list = s_key + l * p.k;
+          if (list[0] < edge) continue;
+          int lo = 0;
+          for (int hi = p.k; lo < hi;) {
+            const int mid = (lo + hi) >> 1;
+            if (list[mid] > s_top[last]) lo = mid + 1; else hi = mid;
+          }
+          for (; lo < p.k; ++lo) {
+            const int i = l * p.k + lo;
+            if (!look(i, list[lo] != 0ull ? list[lo] : any_key(i), __ldcg(elems + i))) break;
+          }
         }
       }
     }
+    if (rows != 0ull) atomicOr(&s_doubt, rows);
     __syncthreads();
-    const unsigned long long rows = s_doubt;
+    return s_doubt;
+  };
+
+  // (One copy of this code for both rankings: two take every call a microsecond more.)
+#pragma unroll 1
+  for (int pass = 0;; ++pass) {
+    const int found = rank_all();
+    if (pass > 0 || p.beams == 1 || sizeof(Score) == 8) break;
+    const unsigned long long rows = in_doubt(found - 1);
     if (rows == 0ull) break;
     for (int b = 0; b < p.beams; ++b) {
       const double ref = s_ref[b];
@@ -705,6 +731,7 @@ beam_join_kernel(SelectParams p) {
       const double sum = sum_again(p.logits + (long long)(row0 + b) * p.ld, p.vocab, ref, s_powers, s_part);
       if (threadIdx.x == 0) s_log[b] = log(sum);
     }
+    __syncthreads();
   }
   for (int i = threadIdx.x; i < p.k; i += kJoinThreads) {
     const size_t at = (size_t)group * p.k + i;
