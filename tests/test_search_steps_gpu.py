@@ -7,6 +7,7 @@ import gc
 import pytest
 import torch
 
+import tiny_configs
 from test_beam_search_gpu import _last_logits, folder_of, llm_for, plain_search, prompts_of
 
 pytestmark = pytest.mark.gpu
@@ -168,3 +169,25 @@ def test_graphs_outlive_another_number_of_prompts():
     assert (wider.buffers.groups, wider.longest, longer.buffers.groups, longer.longest) == (4, 12, 4, 20)
     assert graphs[1] >= graphs[0] and graphs[3] == graphs[2]             # the fourth call replays what the first has captured
     assert llm.beam_search(prompt_token_ids=prompts[:1], params=BeamSearchParams(beam_width=2, max_new_tokens=5)) and llm._beam_runner.width == 2
+
+
+@pytest.mark.parametrize("width,tokens,eos", [(8, 4, ()), (6, 5, (2,)), (16, 3, (0, 4))])
+def test_vocabularies_smaller_than_a_search_is_wide(width, tokens, eos, tmp_path):
+    """One row has fewer continuations than there are beams; several have enough."""
+    import json
+
+    from plain import beam_plain, qwen3_plain
+    from tokamak_b200 import LLM, BeamSearchParams
+    from tokamak_b200.weights import write_random_model
+    raw, init, page = tiny_configs.ALL["C"]
+    write_random_model(str(tmp_path), {**raw, "vocab_size": 7}, dtype="float32", **init)
+    if eos:
+        path = tmp_path / "config.json"
+        path.write_text(json.dumps({**json.loads(path.read_text()), "eos_token_id": list(eos)}))
+    cfg, weights = qwen3_plain.load_folder(str(tmp_path))
+    prompt = [1, 5, 3]
+    llm = LLM(tmp_path, dtype="float32", block_size=page, max_batch_size=width + 1, kv_pool_tokens=4096)
+    found = llm.beam_search(prompt_token_ids=[prompt], params=BeamSearchParams(beam_width=width, max_new_tokens=tokens))[0].hypotheses
+    want, _ = beam_plain.search(lambda t: qwen3_plain.forward_logits(cfg, weights, list(t), torch.float64)[-1], prompt, width=width, max_new=tokens,
+                                stops=eos)
+    assert [h.output_token_ids for h in found] == [t for t, _, _ in want] and len(found) == width

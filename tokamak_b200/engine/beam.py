@@ -169,7 +169,8 @@ class BeamRunner:
         self.cache, self.manager, self.model = step.cache, step.manager, step.model
         self.stops = frozenset(stops)
         self.vocab = self.model.spec.head.vocab_size
-        self.candidates = min(width * (1 + len(self.stops)), self.vocab)
+        # were every EOS token ranked in front of the others in every beam, `width` others are left; a first step has one row's
+        self.candidates = min(width * (1 + len(self.stops)), width * self.vocab)
         self.buffers = BeamBuffers(step, max_groups, width, self.candidates, longest)
         self.stop_tokens = (torch.tensor(sorted(self.stops), dtype=torch.int32, device=step.device) if self.stops else None)
         self.records = list(self.cache._states) + [self.buffers.history.unsqueeze(0)]
@@ -217,8 +218,11 @@ class BeamRunner:
         device = self.step.device
         logits = self.prefill(searches)
         v = b.views(n)
-        ops.beam_select(logits, torch.zeros((n, 1), dtype=torch.float64, device=device), self.candidates,
-                        out=(v["cand_scores"], v["cand_parents"], v["cand_tokens"]), score_dtype=torch.float64)
+        cand = ops.beam_select(logits, torch.zeros((n, 1), dtype=torch.float64, device=device), min(self.candidates, self.vocab),
+                               score_dtype=torch.float64)
+        v["cand_scores"].fill_(-math.inf)
+        for name, part in zip(("cand_scores", "cand_parents", "cand_tokens"), cand):
+            v[name][:, :part.shape[1]] = part
         seats = []
         for s in searches:
             s.beams = [(s.index, i) for i in range(w)]
