@@ -21,7 +21,7 @@
 //
 // Bound by the logits' bytes where there are many: 205 MB (512 rows of 100,003) in 56 us, 3.7 TB/s; what is left are the
 // instructions beside the loads, an exponential and a comparison a logit (44 us without either).  Few rows are bound by
-// latency: 10 us for one row of 151,936, 14 for 32.
+// latency: 10 us for one row of 151,936, 16 for 32.
 //
 // Beams with a score of -inf (or NaN) are not read: their continuations have the key -inf and count from token 0 on.  A NaN
 // logit counts as -inf.  A row with logits of +inf has its mass on these, in equal shares.
